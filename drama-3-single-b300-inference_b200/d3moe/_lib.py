@@ -23,6 +23,8 @@ D3_EWORKSPACE = -3
 D3_EUNSUPPORTED = -4
 D3_DTYPE_BF16 = 0
 D3_DTYPE_F32 = 1
+D3_DTYPE_F16 = 2
+D3_DTYPE_E4M3 = 3
 D3_STATUS_OK = 0
 D3_STATUS_WAIT_TIMEOUT = 1
 D3_STATUS_BAD_ROW = 2
@@ -63,6 +65,62 @@ class D3Rows(ctypes.Structure):
         ("row_slots", _c_void_p),
         ("row_slots_int64", _i32),
         ("padding_start", _i64),
+    ]
+
+
+class D3KvCache(ctypes.Structure):
+    """Mirror of d3_kv_cache_t (one layer's paged keys and values)."""
+
+    _fields_ = [
+        ("k", _c_void_p),
+        ("v", _c_void_p),
+        ("k_page_stride", _i64),
+        ("k_token_stride", _i64),
+        ("k_head_stride", _i64),
+        ("v_page_stride", _i64),
+        ("v_token_stride", _i64),
+        ("v_head_stride", _i64),
+        ("k_scale", _c_void_p),
+        ("v_scale", _c_void_p),
+        ("table", _c_void_p),
+        ("table_stride", _i64),
+        ("sequences", _i32),
+        ("table_pages", _i32),
+        ("num_pages", _i32),
+        ("page_size", _i32),
+        ("heads", _i32),
+        ("dim", _i32),
+        ("dtype", _i32),
+    ]
+
+
+class D3GatedDelta(ctypes.Structure):
+    """Mirror of d3_gated_delta_t (operands of the gated delta rule)."""
+
+    _fields_ = [
+        ("q", _c_void_p),
+        ("k", _c_void_p),
+        ("v", _c_void_p),
+        ("g", _c_void_p),
+        ("beta", _c_void_p),
+        ("out", _c_void_p),
+        ("state", _c_void_p),
+        ("slot", _c_void_p),
+        ("q_stride", _i64),
+        ("k_stride", _i64),
+        ("v_stride", _i64),
+        ("g_stride", _i64),
+        ("beta_stride", _i64),
+        ("out_stride", _i64),
+        ("slot_stride", _i64),
+        ("slots", _i32),
+        ("key_heads", _i32),
+        ("value_heads", _i32),
+        ("key_dim", _i32),
+        ("value_dim", _i32),
+        ("l2norm", _i32),
+        ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
     ]
 
 
@@ -172,6 +230,30 @@ SIGNATURES: dict[str, tuple] = {
         [_c_void_p, _i64, _c_void_p, _c_void_p, _i32, _i32, ctypes.POINTER(D3Experts),
          ctypes.POINTER(D3Experts), _c_void_p, _c_void_p, ctypes.c_float, _c_void_p, _c_void_p,
          _c_void_p, _c_void_p, _size_t, _c_void_p, _c_void_p],
+    ),
+    "d3_kv_append": (
+        _i32,
+        [_c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i32, _i32, _c_void_p, _c_void_p,
+         ctypes.POINTER(D3KvCache), _c_void_p, _c_void_p],
+    ),
+    "d3_copy_pages": (
+        _i32,
+        [_c_void_p, _i32, _i64, _i32, _i64, _i64, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p],
+    ),
+    "d3_paged_attention_workspace_size": (_i32, [_i32, _i32, _i32, _i32, ctypes.POINTER(_size_t)]),
+    "d3_paged_attention": (
+        _i32,
+        [_c_void_p, _i64, _i64, _i32, _i32, _i32, ctypes.POINTER(D3KvCache), _c_void_p, _i32, _i32,
+         ctypes.c_float, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _size_t, _c_void_p, _c_void_p],
+    ),
+    "d3_gated_delta_step": (_i32, [ctypes.POINTER(D3GatedDelta), _i32, _c_void_p, _c_void_p]),
+    "d3_gated_delta_chunk_workspace_size": (
+        _i32, [_i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_size_t)]
+    ),
+    "d3_gated_delta_chunk": (
+        _i32,
+        [ctypes.POINTER(D3GatedDelta), _c_void_p, _i32, _i32, _c_void_p, _c_void_p, _size_t, _c_void_p,
+         _c_void_p],
     ),
     "d3_moe_layer_rows": (
         _i32,

@@ -53,6 +53,8 @@ typedef struct CUstream_st* d3_stream_t; /* == cudaStream_t */
 /* dtype tags used where the reference accepts more than one */
 #define D3_DTYPE_BF16 0
 #define D3_DTYPE_F32 1
+#define D3_DTYPE_F16 2  /* IEEE binary16 (key-value caches and their queries only) */
+#define D3_DTYPE_E4M3 3 /* key-value caches only */
 
 /* Device status word values written by kernels that wait on barriers. */
 #define D3_STATUS_OK 0
@@ -435,6 +437,125 @@ D3_API int d3_ep_unpack_fp8(const uint8_t* recv, int rows, int k, int H, float* 
 D3_API int d3_combine_pairs(const void* rows, const int32_t* inv_rows, const void* weights,
                             int T, int k, int H, const void* shared, const void* gate,
                             int64_t gate_stride, void* out, d3_stream_t stream);
+
+/* ------------------------------------------- sequence memory: key-value pages --
+ * Keys and values of one layer in pages of page_size tokens. Element
+ * [page, token, head, d] of k lies at k + page*k_page_stride +
+ * token*k_token_stride + head*k_head_stride + d (strides in elements, so a
+ * [pages, page_size, heads, dim] and a [pages, heads, page_size, dim] cache
+ * both fit, as does one tensor that holds k and v); the same for v. Row starts
+ * must be 16-byte aligned: base pointers, and strides times the element size.
+ * dtype: D3_DTYPE_BF16, D3_DTYPE_F16, or D3_DTYPE_E4M3 with f32 scales per
+ * head (NULL = 1): the value held is element * scale[head].
+ * table int32 [sequences, table_pages] (row stride table_stride): the page of
+ * token t of sequence b is table[b][t / page_size]. A page number outside
+ * [0, num_pages) sets D3_STATUS_BAD_ROW in the status word where one is given;
+ * such a page is read as page 0 and never written. num_pages must be at least
+ * 1 where anything is read. */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* table;
+  int64_t table_stride;
+  int sequences, table_pages;
+  int num_pages, page_size, heads, dim, dtype;
+} d3_kv_cache_t;
+
+/* Writes new keys and values to their pages: k, v [T, heads, dim] (strides in
+ * elements, rows of dim contiguous and 16-byte aligned) of the cache's dtype,
+ * or bf16 for an e4m3 cache, which takes e4m3(clamp(x / scale[head])). Token t
+ * belongs to sequence seq[t] (NULL: sequence t) at position pos[t]; a token
+ * whose sequence or position is negative is skipped, one whose sequence or
+ * position lies past the table's end is skipped with D3_STATUS_BAD_ROW.
+ * dim a multiple of 8 (16 for e4m3). No two tokens of a call may name the same
+ * place. The reference writes its cache inside prepare_attention
+ * (src/drama3/kernels.py:98-181). */
+D3_API int d3_kv_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride, int dtype, int T,
+                        const int32_t* seq, const int32_t* pos, const d3_kv_cache_t* cache,
+                        int32_t* status, d3_stream_t stream);
+
+/* pool[plane][dst[i]] = pool[plane][src[i]] for every plane and i < n: forks
+ * and compaction of pages (or recurrent-state slots) in all layers at once.
+ * A page is page_bytes contiguous bytes at pool + plane*plane_stride +
+ * page*page_stride (in bytes). No page may be both a source and a destination
+ * of one call, nor a destination twice. A pair with a negative number is
+ * skipped; one with a number >= pages is skipped with D3_STATUS_BAD_ROW. */
+D3_API int d3_copy_pages(void* pool, int planes, int64_t plane_stride, int pages,
+                         int64_t page_stride, int64_t page_bytes, const int32_t* src,
+                         const int32_t* dst, int n, int32_t* status, d3_stream_t stream);
+
+/* Attention of one new token per sequence over its paged keys and values:
+ *   out[b, h] = softmax(scale * q[b, h] . K^T) V,  lse[b, h] = log sum exp
+ * over tokens [max(0, lens[b] - window), lens[b]) of sequence b (window 0: all
+ * of them), with query head h reading key head h / (q_heads / cache heads).
+ * q, out [B, q_heads, dim] in q_dtype (strides in elements, dim contiguous);
+ * q_dtype equals the cache's dtype, or is bf16 for an e4m3 cache. lse f32
+ * [B, q_heads] contiguous, natural logarithm, may be NULL. A sequence of
+ * length 0 gives a zero row and lse = -infinity. lens int32 [B]; max_len is
+ * the host's bound on lens (a longer sequence is read up to max_len, and none
+ * past the table). dim 64, 128 or 256; q_heads a multiple of the cache's heads.
+ * Logits, softmax statistics and sums are fp32. Replaces the reference's paged
+ * decode (src/drama3/model.py:55-141). */
+D3_API int d3_paged_attention_workspace_size(int B, int q_heads, int kv_heads, int dim,
+                                             size_t* bytes);
+D3_API int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride, int q_dtype,
+                              int B, int q_heads, const d3_kv_cache_t* cache, const int32_t* lens,
+                              int max_len, int window, float scale, void* out,
+                              int64_t out_row_stride, int64_t out_head_stride, float* lse,
+                              void* workspace, size_t workspace_bytes, int32_t* status,
+                              d3_stream_t stream);
+
+/* ----------------------------------------------- sequence memory: gated delta --
+ * The gated delta rule. Per sequence and value head h, with state S f32
+ * [key_dim, value_dim], each token does
+ *   S <- exp(g) S;  S <- S + k (beta (v - S^T k))^T;  out = S^T (scale q)
+ * where q and k are key head h / (value_heads / key_heads), divided by
+ * sqrt(|x|^2 + eps) first when l2norm is not 0. q, k bf16 [T, key_heads,
+ * key_dim]; v, out bf16 [T, value_heads, value_dim] (token strides in elements,
+ * heads and dims contiguous); g (log decay, <= 0), beta f32 [T, value_heads]
+ * (token strides in elements). state f32 [slots, value_heads, key_dim,
+ * value_dim] (slot stride in elements) is updated in place. key_dim and
+ * value_dim 64 or 128; q, k, v, out rows and the state 16-byte aligned.
+ * slot int32 [n] names each sequence's state (NULL: slot i for sequence i). A
+ * sequence with a negative slot is left out (its out rows are zero), as is,
+ * with D3_STATUS_BAD_ROW, one whose slot is >= slots. No two sequences of a
+ * call may share a slot.
+ * The reference runs these from SGLang (src/drama3/gdn.py:8-195). */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* g;
+  const float* beta;
+  void* out;
+  float* state;
+  const int32_t* slot;
+  int64_t q_stride, k_stride, v_stride, g_stride, beta_stride, out_stride, slot_stride;
+  int slots, key_heads, value_heads, key_dim, value_dim;
+  int l2norm;
+  float scale, eps;
+} d3_gated_delta_t;
+
+/* One new token for each of n sequences (row i of q, k, v, g, beta, out). */
+D3_API int d3_gated_delta_step(const d3_gated_delta_t* args, int n, int32_t* status,
+                               d3_stream_t stream);
+
+/* Packed prompts: rows [cu[i], cu[i+1]) of q, k, v, g, beta and out are sequence
+ * i's tokens (cu int32 [n+1] on the device, non-decreasing, cu[0] >= 0, cu[n]
+ * <= T; rows that belong to no sequence are not written). fresh (uint8 [n], may
+ * be NULL): a sequence whose entry is not 0 starts from a zero state instead of
+ * its slot's. A sequence without tokens leaves its state as it is, or zeroes it
+ * when fresh. */
+D3_API int d3_gated_delta_chunk_workspace_size(int T, int n, int value_heads, int key_dim,
+                                               int value_dim, size_t* bytes);
+D3_API int d3_gated_delta_chunk(const d3_gated_delta_t* args, const int32_t* cu, int T, int n,
+                                const uint8_t* fresh, void* workspace, size_t workspace_bytes,
+                                int32_t* status, d3_stream_t stream);
 
 /* Profiling hook, off by default: while set, d3_moe_experts / d3_moe_layer
  * calls made by the calling thread (the setting is per host thread) record
