@@ -1,16 +1,41 @@
 // Attention of one new token per sequence over paged keys and values.
 //
-// One CTA per (sequence, key head, group of up to 8 of its query heads). Each
-// of 8 warps takes every eighth key: its lanes split the row, a dot product
-// per query head is joined by shuffles, and the warp keeps the running
-// maximum, sum and output row of each head (fp32). The warps join at the end.
+//   s_j = scale q.k_j,  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
+//
+// Each key and value is read once and used by the query heads that share it,
+// a few flops per byte: the kernel is bound by HBM, and everything else has to
+// hide behind the loads.
+//
+// Work. A unit is a (sequence, key head, group of query heads); its keys are
+// cut into tiles of 4 * NK. All units' tiles form one line, and each CTA of a
+// persistent grid (one per SM) takes an equal share of it, so ragged lengths
+// balance by themselves and a single long sequence uses every SM. A CTA's share
+// may end inside a unit: such parts leave (max, sum, output row) in the
+// workspace, and a second kernel joins them in CTA order (no atomics, so equal
+// inputs give equal bits).
+//
+// Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
+// tile, loads them with cp.async into its own ring of shared-memory stages
+// (no barrier between warps), and works with mma.sync m16n8k16: queries are
+// the 16 rows of A, keys the columns of B for the logits, and the probabilities
+// go back in as A from the registers that hold them (the accumulator layout is
+// the A layout). tcgen05 has nothing to add here: its 128-row tile would be 1/16
+// used. With up to 8 query heads per key head only rows 0-7 of A are needed, and
+// rows 8-15 carry, for bf16, the part of each probability that its rounding
+// to bf16 lost: the products are then exact to 2^-17 at no cost.
+//
+// An e4m3 cache is widened to f16 in registers (exact). Its queries are scaled by
+// a power of two per row into f16's range (exact for every element within 2^-14
+// of the row's largest, error below 2^-25 of that otherwise).
 #include "kv_cache.cuh"
 
 namespace d3 {
 namespace {
 
-constexpr int kAttnWarps = 8;
-constexpr int kAttnHeads = 8;  // query heads of one CTA
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct AttnArgs {
   const uint16_t* q;
@@ -26,125 +51,615 @@ struct AttnArgs {
   const int32_t* table;
   int64_t table_stride;
   const int32_t* lens;
-  int max_len, window, num_pages, page_size, q_heads, group;
+  int B, max_len, window, num_pages, page_size, q_heads, group;
+  int parts, units;  // query-head groups per key head; units per sequence
   float scale;
+  float* partial;    // [grid][2] records of ROWS * (D + 2) floats
+  int grid;          // CTAs of the main kernel
   int32_t* status;
 };
 
-template <int DT>
-__device__ __forceinline__ float half_to_f32(uint16_t b) {
-  if constexpr (DT == D3_DTYPE_F16) return __half2float(__ushort_as_half(b));
-  return bf16_bits_to_f32(b);
+// Sizes of one variant. WIDE: 16 query heads per unit, else 8.
+template <int DT, int D, bool WIDE>
+struct AttnShape {
+  static constexpr int kElem = DT == D3_DTYPE_E4M3 ? 1 : 2;
+  static constexpr int kRowBytes = D * kElem;
+  // keys of one warp and stage: about 8 KB of keys and as much of values
+  static constexpr int kNK = 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;
+  static constexpr int kTile = kNK * kAttnWarps;
+  static constexpr int kRows = WIDE ? 16 : 8;
+  static constexpr int kHalf = kNK * kRowBytes;  // bytes of a stage's keys
+  static constexpr int kStage = 2 * kHalf;
+  static constexpr int kJoin = kAttnWarps * kRows * D * 4;  // the warps' output rows
+  static constexpr int kRing = kAttnWarps * kStage;
+  static constexpr int kStages = 3 * kRing + kJoin + 2048 <= 227 * 1024 ? 3 : 2;
+  static constexpr int kSmem = kStages * kRing + kJoin + 2048;
+  static constexpr int kRecord = kRows * (D + 2);  // floats of a partial result
+};
+
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-// E = dim / 32 consecutive elements of a row, as fp32.
-template <int DT, int E>
-__device__ __forceinline__ void load_row_part(const uint8_t* row, int lane, float (&f)[E]) {
-  if constexpr (DT == D3_DTYPE_E4M3) {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row + lane * E);
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const uint32_t h = e4m3x2_to_f16x2(p[i]);
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      f[2 * i] = x.x;
-      f[2 * i + 1] = x.y;
-    }
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1,
+                                                  uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+// c += A(16x16, row) * B(16x8, col) for bf16 or f16 operands.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
   } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) f[i] = half_to_f32<DT>(p[i]);
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
   }
 }
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) paged_attention_kernel(const AttnArgs a) {
-  constexpr int E = D / 32;
-  constexpr int QT = DT == D3_DTYPE_F16 ? D3_DTYPE_F16 : D3_DTYPE_BF16;
-  __shared__ float s_m[kAttnWarps][kAttnHeads], s_l[kAttnWarps][kAttnHeads];
-  __shared__ float s_o[kAttnWarps][D];
-  pdl_enter();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z, kh = blockIdx.y;
-  const int h0 = kh * a.group + blockIdx.x * kAttnHeads;
-  const int nh = min(kAttnHeads, (kh + 1) * a.group - h0);
-  const int len = max(0, min(__ldg(a.lens + b), a.max_len));
-  const int begin = a.window > 0 ? max(0, len - a.window) : 0;
-  const float ks = a.scale * (a.k_scale ? __ldg(a.k_scale + kh) : 1.0f);
-  float q[kAttnHeads][E], o[kAttnHeads][E], m[kAttnHeads], l[kAttnHeads];
-#pragma unroll
-  for (int h = 0; h < kAttnHeads; ++h) {
-    m[h] = -INFINITY;
-    l[h] = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      o[h][i] = 0.f;
-      q[h][i] = h < nh ? half_to_f32<QT>(a.q[b * a.q_row + (h0 + h) * a.q_head + lane * E + i]) : 0.f;
-    }
+template <bool BF16>
+__device__ __forceinline__ float unpack16(uint16_t b) {
+  if constexpr (BF16) return bf16_bits_to_f32(b);
+  return __half2float(__ushort_as_half(b));
+}
+
+// Byte offset of 16-byte piece c of row r in a stage: pieces are permuted so
+// that the 8 rows of an ldmatrix tile fall into different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint32_t ring_at(int r, int c) {
+  constexpr int kPieces = ROW_BYTES / 16;
+  const int x = kPieces >= 8 ? (r & 7) : ((r >> 1) & 3);  // 64-byte rows share a 128-byte line
+  return r * ROW_BYTES + ((c ^ x) << 4);
+}
+
+__device__ __forceinline__ int seq_begin(const AttnArgs& a, int len) {
+  return a.window > 0 ? max(0, len - a.window) : 0;
+}
+__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
+  return max(0, min(__ldg(a.lens + b), a.max_len));
+}
+template <int TILE>
+__device__ __forceinline__ int seq_tiles(const AttnArgs& a, int b) {
+  const int len = seq_len(a, b);
+  return (len - seq_begin(a, len) + TILE - 1) / TILE;
+}
+
+// Tiles of one CTA: an equal share of the line, at least kMinShare.
+constexpr int kMinShare = 2;
+__device__ __forceinline__ int64_t cta_share(int64_t total, int grid) {
+  const int64_t s = (total + grid - 1) / grid;
+  return s < kMinShare ? kMinShare : s;
+}
+
+// Sums over the sequences with 128 threads: the tiles of all units of all
+// sequences, and each thread's exclusive prefix over its own run of `per`
+// sequences. scratch: 8 values of shared memory.
+template <int TILE>
+__device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int64_t* scratch, int64_t& mine,
+                                          int64_t& before, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = threadIdx.x * per + i;
+    if (b < a.B) mine += seq_tiles<TILE>(a, b);
   }
-  for (int t = begin + warp; t < len; t += kAttnWarps) {
-    int page = __ldg(a.table + b * a.table_stride + t / a.page_size);
-    if (page < 0 || page >= a.num_pages) {
-      if (a.status) atomicExch(a.status, kDevBadRow);
-      page = 0;
-    }
-    const int off = t % a.page_size;
-    float kf[E], vf[E];
-    load_row_part<DT, E>(a.k + page * a.k_page + off * a.k_token + kh * a.k_head, lane, kf);
-    load_row_part<DT, E>(a.v + page * a.v_page + off * a.v_token + kh * a.v_head, lane, vf);
+  mine *= a.units;
+  int64_t x = mine;
 #pragma unroll
-    for (int h = 0; h < kAttnHeads; ++h) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(q[h][i], kf[i], s);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= ks;
-      const float mn = fmaxf(m[h], s);
-      const float base = mn == -INFINITY ? 0.f : mn;  // a logit of -inf adds nothing
-      const float c = expf(m[h] - base), p = expf(s - base);
-      m[h] = mn;
-      l[h] = l[h] * c + p;
-#pragma unroll
-      for (int i = 0; i < E; ++i) o[h][i] = fmaf(p, vf[i], o[h][i] * c);
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  if (lane == 0)
-    for (int h = 0; h < kAttnHeads; ++h) {
-      s_m[warp][h] = m[h];
-      s_l[warp][h] = l[h];
-    }
-  const float vs = a.v_scale ? __ldg(a.v_scale + kh) : 1.0f;
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  before = x - mine;
+  total = 0;
 #pragma unroll
-  for (int h = 0; h < kAttnHeads; ++h) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = o[h][i];
-    __syncthreads();
-    if (h >= nh) continue;
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, s_m[w][h]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int w = 0; w < kAttnWarps; ++w) sum += s_l[w][h] * expf(s_m[w][h] - base);
-    for (int d = threadIdx.x; d < D; d += kAttnWarps * 32) {
-      float x = 0.f;
-      for (int w = 0; w < kAttnWarps; ++w) x += s_o[w][d] * expf(s_m[w][h] - base);
-      x = sum == 0.f ? 0.f : x / sum * vs;  // a NaN stays one
-      uint16_t r;
-      if constexpr (QT == D3_DTYPE_F16) r = __half_as_ushort(__float2half_rn(x));
-      else r = __bfloat16_as_ushort(__float2bfloat16_rn(x));
-      a.out[b * a.out_row + (h0 + h) * a.out_head + d] = r;
-    }
-    if (a.lse && threadIdx.x == 0)
-      a.lse[static_cast<int64_t>(b) * a.q_heads + h0 + h] = sum == 0.f ? -INFINITY : logf(sum) + top;
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
   }
 }
 
-template <int DT>
-void launch_attention(const AttnArgs& a, int D, dim3 grid, cudaStream_t s) {
-  const dim3 block(kAttnWarps * 32);
-  if (D == 64) launch_kernel(paged_attention_kernel<DT, 64>, grid, block, 0, s, a);
-  else if (D == 128) launch_kernel(paged_attention_kernel<DT, 128>, grid, block, 0, s, a);
-  else launch_kernel(paged_attention_kernel<DT, 256>, grid, block, 0, s, a);
+// A place on the line: unit `unit` of sequence b, tile `tile` of its `tiles`.
+template <int TILE>
+struct Cursor {
+  int b, unit, tile, tiles, len, begin;
+  __device__ __forceinline__ void enter(const AttnArgs& a) {
+    len = seq_len(a, b);
+    begin = seq_begin(a, len);
+    tiles = (len - begin + TILE - 1) / TILE;
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++unit < a.units) return;
+    unit = 0;
+    do {
+      if (++b >= a.B) return;
+      enter(a);
+    } while (tiles == 0);
+  }
+};
+
+template <int DT, int D, bool WIDE>
+__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const AttnArgs a) {
+  using Sh = AttnShape<DT, D, WIDE>;
+  constexpr bool BF16 = DT == D3_DTYPE_BF16;        // type of the matrix products
+  constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
+  constexpr bool SPLIT = BF16 && !WIDE;             // rows 8-15 carry the rounding's rest
+  constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kStages, ROWS = Sh::kRows;
+  constexpr int KS = D / 16, NT = NK / 8, DT8 = D / 8;
+  constexpr int PIECES = RB / 16, RPL = (NK + 31) / 32;  // rows whose page a lane looks up
+  extern __shared__ __align__(1024) uint8_t smem[];
+  float* join = reinterpret_cast<float*>(smem + S * Sh::kRing);
+  float* stat = reinterpret_cast<float*>(smem + S * Sh::kRing + Sh::kJoin);  // [warps][2][16]
+  int64_t* scratch = reinterpret_cast<int64_t*>(stat + kAttnWarps * 32);
+  int* start = reinterpret_cast<int*>(scratch + 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int quad = lane >> 2, t4 = lane & 3;
+
+  pdl_wait();
+  pdl_trigger();  // after the wait: the joining kernel may read lens before it waits itself
+
+  // where this CTA's share of the line begins
+  const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
+  int64_t mine, before, total;
+  line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
+  const int64_t share = cta_share(total, a.grid);
+  const int64_t first = blockIdx.x * share;
+  if (first >= total) return;
+  const int count = static_cast<int>(min(share, total - first));
+  if (first >= before && first < before + mine) {
+    int64_t at = before;
+    for (int i = 0; i < per; ++i) {
+      const int b = tid * per + i;
+      const int64_t n = static_cast<int64_t>(seq_tiles<Sh::kTile>(a, b)) * a.units;
+      if (first < at + n) {
+        const int tiles = static_cast<int>(n / a.units);
+        start[0] = b;
+        start[1] = static_cast<int>((first - at) / tiles);
+        start[2] = static_cast<int>((first - at) % tiles);
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Cursor<Sh::kTile> cur;
+  cur.b = start[0];
+  cur.unit = start[1];
+  cur.tile = start[2];
+  cur.enter(a);
+  Cursor<Sh::kTile> ld = cur;
+
+  const uint32_t ring = smem_u32(smem) + warp * Sh::kStage;  // + stage * kRing
+
+  // pages of the rows of tile `ld` that this lane looks up (row = lane + 32 i)
+  int page[RPL], off[RPL];
+  auto look_up = [&]() {
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) {
+      const int j = ld.begin + ld.tile * Sh::kTile + warp * NK + lane + 32 * i;
+      page[i] = -1;
+      if (lane + 32 * i < NK && j < ld.len) {
+        const int slot = j / a.page_size;
+        off[i] = j - slot * a.page_size;
+        int p = __ldg(a.table + ld.b * a.table_stride + slot);
+        if (p < 0 || p >= a.num_pages) {
+          if (a.status) atomicExch(a.status, kDevBadRow);
+          p = 0;
+        }
+        page[i] = p;
+      }
+    }
+  };
+  // copies this warp's rows of tile `ld` into stage s; rows past the sequence's
+  // end are zeroed (what the cache holds there may be anything, NaN included)
+  auto load = [&](int s) {
+    const int head = ld.unit / a.parts;
+    const uint8_t* kb = a.k + head * a.k_head;
+    const uint8_t* vb = a.v + head * a.v_head;
+    const uint32_t dst = ring + s * Sh::kRing;
+#pragma unroll
+    for (int it = 0; it < NK * PIECES / 32; ++it) {
+      const int idx = it * 32 + lane, r = idx / PIECES, c = idx % PIECES;
+      const int from = (it * 32 / PIECES) >> 5;  // which of the lanes' rows (uniform)
+      int p, o;
+      if constexpr (RPL == 1) {
+        p = __shfl_sync(0xffffffffu, page[0], r);
+        o = __shfl_sync(0xffffffffu, off[0], r);
+      } else {
+        p = __shfl_sync(0xffffffffu, page[from], r & 31);
+        o = __shfl_sync(0xffffffffu, off[from], r & 31);
+      }
+      const bool take = p >= 0;
+      const int64_t pp = take ? p : 0, oo = take ? o : 0;
+      const uint32_t at = ring_at<RB>(r, c);
+      cp_async_16_zfill(dst + at, kb + pp * a.k_page + oo * a.k_token + c * 16, take);
+      cp_async_16_zfill(dst + Sh::kHalf + at, vb + pp * a.v_page + oo * a.v_token + c * 16, take);
+    }
+  };
+
+  int loaded = 0;
+  look_up();
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) {
+    if (loaded < count) {
+      load(s);
+      if (++loaded < count) {
+        ld.next(a);
+        look_up();
+      }
+    }
+    cp_async_commit();
+  }
+
+  uint32_t qf[KS][WIDE ? 4 : 2];
+  float o[DT8][4], m[WIDE ? 2 : 1], l[WIDE ? 2 : 1];
+  float lg[WIDE ? 2 : 1];  // logit in units of log2 per product
+  bool opened = false, whole = false;
+  int seg_slot = 0;
+  for (int i = 0; i < count; ++i) {
+    const int head = cur.unit / a.parts;
+    const int h0 = head * a.group + (cur.unit % a.parts) * ROWS;
+    const int nh = min(ROWS, (head + 1) * a.group - h0);
+    if (!opened) {
+      opened = true;
+      whole = cur.tile == 0;
+      seg_slot = i > 0;
+#pragma unroll
+      for (int d = 0; d < DT8; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
+#pragma unroll
+      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+        m[w] = -INFINITY;
+        l[w] = 0.f;
+        const int r = quad + 8 * w;
+        const uint16_t* row = a.q + cur.b * a.q_row + static_cast<int64_t>(h0 + (r < nh ? r : 0)) * a.q_head;
+        float ks = a.scale * kLog2e;
+        if constexpr (DT == D3_DTYPE_E4M3) {
+          // the row's largest element decides its power of two
+          float top = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top = fmaxf(top, fabsf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + x))));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          int e = 0;
+          if (top > 0.f && isfinite(top)) frexpf(top, &e);
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float lo = ldexpf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + 2 * x)), -e);
+              const float hi = ldexpf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + 2 * x + 1)), -e);
+              qf[s][WIDE ? 2 * x + w : x] = r < nh ? pack16<false>(lo, hi) : 0u;
+            }
+          ks = ldexpf(ks * (a.k_scale ? __ldg(a.k_scale + head) : 1.0f), e);
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint16_t* p = row + 16 * s + 2 * t4 + 8 * x;
+              const uint32_t two = static_cast<uint32_t>(__ldg(p)) | (static_cast<uint32_t>(__ldg(p + 1)) << 16);
+              qf[s][WIDE ? 2 * x + w : x] = r < nh ? two : 0u;
+            }
+        }
+        lg[w] = ks;
+      }
+    }
+    // the next stage's loads go out before this stage's work
+    if (loaded < count) {
+      load((i + S - 1) % S);
+      if (++loaded < count) {
+        ld.next(a);
+        look_up();
+      }
+    }
+    cp_async_commit();
+    cp_async_wait<S - 1>();
+    __syncwarp();
+
+    const uint32_t ks = ring + (i % S) * Sh::kRing, vs = ks + Sh::kHalf;
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
+    // logits: rows of K are the columns of B
+    const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
+    if constexpr (DT == D3_DTYPE_E4M3) {
+#pragma unroll
+      for (int c = 0; c < KS; c += 2)  // 16 bytes of a row are one k step
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b[4];
+          ldmatrix_x4(ks + ring_at<RB>(n * 8 + mtop * 8 + mrow, c + mhi), b[0], b[1], b[2], b[3]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y)    // k step
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // 8 keys
+              const uint32_t w = b[2 * x + y];
+              const uint32_t b0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w)), b1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
+              if constexpr (WIDE) mma_16816<false>(s[n + x], qf[c + y][0], qf[c + y][1], qf[c + y][2], qf[c + y][3], b0, b1);
+              else mma_16816<false>(s[n + x], qf[c + y][0], 0u, qf[c + y][1], 0u, b0, b1);
+            }
+        }
+    } else {
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b[4];
+          ldmatrix_x4(ks + ring_at<RB>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if constexpr (WIDE) mma_16816<BF16>(s[n + x], qf[c][0], qf[c][1], qf[c][2], qf[c][3], b[2 * x], b[2 * x + 1]);
+            else mma_16816<BF16>(s[n + x], qf[c][0], 0u, qf[c][1], 0u, b[2 * x], b[2 * x + 1]);
+          }
+        }
+    }
+    // keys past the end take no part
+    const int left = cur.len - (cur.begin + cur.tile * Sh::kTile + warp * NK);
+    uint32_t pf[NT][2];  // probabilities as A operands: [8 keys][rows 0-7, rows 8-15]
+#pragma unroll
+    for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float& y = s[n][2 * w + x];
+          y = n * 8 + 2 * t4 + x < left ? y * lg[w] : -INFINITY;
+          top = fmaxf(top, y);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float mn = fmaxf(m[w], top);
+      if (__any_sync(0xffffffffu, mn > m[w])) {  // some row has a new maximum: rescale what it has
+        const float c = exp2f(m[w] - (mn == -INFINITY ? 0.f : mn));
+        l[w] *= c;
+#pragma unroll
+        for (int d = 0; d < DT8; ++d) {
+          o[d][2 * w] *= c;
+          o[d][2 * w + 1] *= c;
+          if constexpr (SPLIT) {
+            o[d][2] *= c;
+            o[d][3] *= c;
+          }
+        }
+      }
+      m[w] = mn;
+      const float base = mn == -INFINITY ? 0.f : mn;  // no key yet, or only logits of -inf
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float p0 = exp2f(s[n][2 * w] - base), p1 = exp2f(s[n][2 * w + 1] - base);
+        l[w] += p0 + p1;
+        const uint32_t hi = pack16<BF16>(p0, p1);
+        pf[n][w] = hi;
+        if constexpr (SPLIT)
+          pf[n][1] = pack16<true>(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+        else if constexpr (!WIDE)
+          pf[n][1] = 0u;
+      }
+    }
+    // out += P V
+    if constexpr (DT == D3_DTYPE_E4M3) {
+#pragma unroll
+      for (int n = 0; n < NT; n += 2)
+#pragma unroll
+        for (int c = 0; c < D / 16; c += 2) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(vs + ring_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            // a 16-bit unit holds two neighbouring columns of a key: even and
+            // odd columns go to two products
+            const uint32_t w0 = b[2 * y], w1 = b[2 * y + 1];
+            const uint32_t e0 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0020)));
+            const uint32_t e1 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0020)));
+            const uint32_t d0 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0031)));
+            const uint32_t d1 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0031)));
+            mma_16816<false>(o[2 * (c + y)], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], e0, e1);
+            mma_16816<false>(o[2 * (c + y) + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], d0, d1);
+          }
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; n += 2)
+#pragma unroll
+        for (int c = 0; c < DT8; c += 2) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(vs + ring_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
+          mma_16816<BF16>(o[c], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[0], b[1]);
+          mma_16816<BF16>(o[c + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[2], b[3]);
+        }
+    }
+    __syncwarp();  // every lane has read this stage before it is loaded again
+
+    const bool last = cur.tile + 1 == cur.tiles;
+    if (last || i + 1 == count) {
+      // join the warps: (max, sum) and output rows through shared memory
+      opened = false;
+#pragma unroll
+      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
+        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
+        if (t4 == 0) {
+          stat[warp * 32 + quad + 8 * w] = m[w];
+          stat[warp * 32 + 16 + quad + 8 * w] = l[w];
+        }
+        float* row = join + (warp * ROWS + quad + 8 * w) * D;
+#pragma unroll
+        for (int d = 0; d < DT8; ++d) {
+          float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
+          if constexpr (SPLIT) {
+            x0 += o[d][2];
+            x1 += o[d][3];
+          }
+          if constexpr (DT == D3_DTYPE_E4M3) {
+            row[(d >> 1) * 16 + 4 * t4 + (d & 1)] = x0;
+            row[(d >> 1) * 16 + 4 * t4 + 2 + (d & 1)] = x1;
+          } else {
+            *reinterpret_cast<float2*>(row + d * 8 + 2 * t4) = make_float2(x0, x1);
+          }
+        }
+      }
+      __syncthreads();
+      whole = whole && last;
+      float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
+      const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
+      for (int e = tid * 4; e < ROWS * D; e += kAttnThreads * 4) {
+        const int r = e / D, d = e % D;
+        if (r >= nh) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, stat[w * 32 + r]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x[4] = {};
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+          const float f = exp2f(stat[w * 32 + r] - base);
+          sum += f * stat[w * 32 + 16 + r];
+          const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * D + d);
+          x[0] = fmaf(f, y.x, x[0]);
+          x[1] = fmaf(f, y.y, x[1]);
+          x[2] = fmaf(f, y.z, x[2]);
+          x[3] = fmaf(f, y.w, x[3]);
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : vsc / sum;  // a NaN stays one
+          const uint2 two = make_uint2(pack16<QBF16>(x[0] * inv, x[1] * inv), pack16<QBF16>(x[2] * inv, x[3] * inv));
+          uint16_t* at = a.out + cur.b * a.out_row + (h0 + r) * a.out_head + d;
+          at[0] = static_cast<uint16_t>(two.x);
+          at[1] = static_cast<uint16_t>(two.x >> 16);
+          at[2] = static_cast<uint16_t>(two.y);
+          at[3] = static_cast<uint16_t>(two.y >> 16);
+          if (a.lse && d == 0)
+            a.lse[static_cast<int64_t>(cur.b) * a.q_heads + h0 + r] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
+        } else {
+          *reinterpret_cast<float4*>(rec + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+          if (d == 0) {
+            rec[ROWS * D + r] = top;
+            rec[ROWS * D + ROWS + r] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (i + 1 < count) cur.next(a);
+  }
+  cp_async_wait<0>();
+}
+
+// One CTA per unit: units without keys get zeros, units that several CTAs
+// shared are joined from their records in CTA order.
+template <int DT, int D, bool WIDE>
+__global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(const AttnArgs a) {
+  using Sh = AttnShape<DT, D, WIDE>;
+  constexpr bool QBF16 = DT != D3_DTYPE_F16;
+  constexpr int ROWS = Sh::kRows;
+  __shared__ int64_t scratch[8], found;
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / a.units, unit = blockIdx.x % a.units;
+  const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
+  pdl_trigger();
+  int64_t mine, before, total;
+  line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
+  const int tiles = seq_tiles<Sh::kTile>(a, b);
+  if (b / per == tid) {
+    int64_t at = before;
+    for (int x = tid * per; x < b; ++x) at += static_cast<int64_t>(seq_tiles<Sh::kTile>(a, x)) * a.units;
+    found = at + static_cast<int64_t>(unit) * tiles;
+  }
+  __syncthreads();
+  const int64_t share = cta_share(total, a.grid);
+  const int64_t lo = found, hi = lo + tiles;  // the unit's tiles on the line
+  const int c0 = static_cast<int>(lo / share), c1 = static_cast<int>((hi - 1) / share);
+  // every CTA waits: a kernel after this one waits for this grid only, which
+  // must not be complete before the main kernel is
+  pdl_wait();
+  if (tiles > 0 && c0 == c1) return;
+  const int head = unit / a.parts;
+  const int h0 = head * a.group + (unit % a.parts) * ROWS;
+  const int nh = min(ROWS, (head + 1) * a.group - h0);
+  const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
+  for (int e = tid * 4; e < nh * D; e += kAttnThreads * 4) {
+    const int r = e / D, d = e % D;
+    float top = -INFINITY, sum = 0.f, x[4] = {};
+    if (tiles > 0) {
+      for (int c = c0; c <= c1; ++c) {
+        const float* rec = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 && lo % share != 0)) * Sh::kRecord;
+        const float mc = __ldcg(rec + ROWS * D + r), lc = __ldcg(rec + ROWS * D + ROWS + r);
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(rec + r * D + d));
+        const float mn = fmaxf(top, mc), base = mn == -INFINITY ? 0.f : mn;
+        const float f = exp2f(top - base), g = exp2f(mc - base);
+        top = mn;
+        sum = sum * f + lc * g;
+        x[0] = x[0] * f + y.x * g;
+        x[1] = x[1] * f + y.y * g;
+        x[2] = x[2] * f + y.z * g;
+        x[3] = x[3] * f + y.w * g;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : vsc / sum;
+    const uint2 two = make_uint2(pack16<QBF16>(x[0] * inv, x[1] * inv), pack16<QBF16>(x[2] * inv, x[3] * inv));
+    uint16_t* at = a.out + b * a.out_row + (h0 + r) * a.out_head + d;
+    at[0] = static_cast<uint16_t>(two.x);
+    at[1] = static_cast<uint16_t>(two.x >> 16);
+    at[2] = static_cast<uint16_t>(two.y);
+    at[3] = static_cast<uint16_t>(two.y >> 16);
+    if (a.lse && d == 0)
+      a.lse[static_cast<int64_t>(b) * a.q_heads + h0 + r] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
+  }
+}
+
+template <int DT, int D, bool WIDE>
+int launch_attention(AttnArgs& a, cudaStream_t s) {
+  using Sh = AttnShape<DT, D, WIDE>;
+  static bool ready[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(paged_attention_kernel<DT, D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
+      return check_launch("d3_paged_attention");
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  launch_kernel(paged_attention_kernel<DT, D, WIDE>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
+  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.units)), dim3(kAttnThreads), 0, s, a);
+  return check_launch("d3_paged_attention");
+}
+
+template <int DT, bool WIDE>
+int launch_dim(AttnArgs& a, int D, cudaStream_t s) {
+  if (D == 64) return launch_attention<DT, 64, WIDE>(a, s);
+  if (D == 128) return launch_attention<DT, 128, WIDE>(a, s);
+  return launch_attention<DT, 256, WIDE>(a, s);
 }
 
 }  // namespace
@@ -157,7 +672,8 @@ extern "C" int d3_paged_attention_workspace_size(int B, int q_heads, int kv_head
   D3_REQUIRE(B >= 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0,
              "query heads must be a multiple of key heads");
   D3_REQUIRE(dim == 64 || dim == 128 || dim == 256, "head dim must be 64, 128 or 256");
-  *bytes = 0;
+  const int rows = q_heads / kv_heads > 8 ? 16 : 8;
+  *bytes = static_cast<size_t>(sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
   return D3_OK;
 }
 
@@ -174,8 +690,9 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
              "queries of dtype %d for a cache of dtype %d", q_dtype, cache->dtype);
   D3_REQUIRE(max_len >= 0 && window >= 0, "negative length bound or window");
   D3_REQUIRE(cache->sequences == B, "the page table must have one row per query");
-  if (workspace_bytes < need || (need && !workspace))
+  if (workspace_bytes < need || !workspace)
     return set_error(D3_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  D3_REQUIRE(aligned(workspace, 16), "the workspace must be 16-byte aligned");
   if (B == 0) return D3_OK;
   D3_REQUIRE(q && out && lens, "NULL operand");
   const int64_t held = static_cast<int64_t>(cache->table_pages) * cache->page_size;
@@ -203,18 +720,25 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   a.table = cache->table;
   a.table_stride = cache->table_stride;
   a.lens = lens;
+  a.B = B;
   a.window = window;
   a.num_pages = cache->num_pages;
   a.page_size = cache->page_size;
   a.q_heads = q_heads;
   a.group = q_heads / cache->heads;
+  const bool wide = a.group > 8;  // 16 heads share a read of the keys where there are more than 8
+  a.parts = (a.group + (wide ? 15 : 7)) / (wide ? 16 : 8);
+  a.units = cache->heads * a.parts;
   a.scale = scale;
+  a.partial = static_cast<float*>(workspace);
+  a.grid = sm_count();
   a.status = status;
-  const dim3 grid((a.group + kAttnHeads - 1) / kAttnHeads, cache->heads, B);
-  D3_REQUIRE(B <= 65535 && cache->heads <= 65535, "batch or heads too large");
+  D3_REQUIRE(static_cast<int64_t>(B) * a.units <= 0x7fffffff, "batch or heads too large");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (cache->dtype == D3_DTYPE_BF16) launch_attention<D3_DTYPE_BF16>(a, cache->dim, grid, s);
-  else if (cache->dtype == D3_DTYPE_F16) launch_attention<D3_DTYPE_F16>(a, cache->dim, grid, s);
-  else launch_attention<D3_DTYPE_E4M3>(a, cache->dim, grid, s);
-  return check_launch("d3_paged_attention");
+  const int D = cache->dim;
+  switch (cache->dtype) {
+    case D3_DTYPE_BF16: return wide ? launch_dim<D3_DTYPE_BF16, true>(a, D, s) : launch_dim<D3_DTYPE_BF16, false>(a, D, s);
+    case D3_DTYPE_F16: return wide ? launch_dim<D3_DTYPE_F16, true>(a, D, s) : launch_dim<D3_DTYPE_F16, false>(a, D, s);
+    default: return wide ? launch_dim<D3_DTYPE_E4M3, true>(a, D, s) : launch_dim<D3_DTYPE_E4M3, false>(a, D, s);
+  }
 }
