@@ -7,16 +7,16 @@
 // hide behind the loads.
 //
 // Work. A unit is a (sequence, key head, group of query heads); its keys are
-// cut into tiles of 4 * NK. All units' tiles form one line, and each CTA of a
+// cut into tiles of 8 * NK. All units' tiles form one line, and each CTA of a
 // persistent grid (one per SM) takes an equal share of it, so ragged lengths
 // balance by themselves and a single long sequence uses every SM. A CTA's share
 // may end inside a unit: such parts leave (max, sum, output row) in the
 // workspace, and a second kernel joins them in CTA order (no atomics, so equal
 // inputs give equal bits).
 //
-// Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
-// tile, loads them with cp.async into its own ring of shared-memory stages
-// (no barrier between warps), and works with mma.sync m16n8k16: queries are
+// Inside a CTA 8 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
+// tile, loads them with cp.async into its own ring of shared-memory slots (keys
+// and values of a tile are two slots; no barrier between warps), and works with mma.sync m16n8k16: queries are
 // the 16 rows of A, keys the columns of B for the logits, and the probabilities
 // go back in as A from the registers that hold them (the accumulator layout is
 // the A layout). tcgen05 has nothing to add here: its 128-row tile would be 1/16
@@ -32,7 +32,7 @@
 namespace d3 {
 namespace {
 
-constexpr int kAttnWarps = 4;
+constexpr int kAttnWarps = 8;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -64,16 +64,19 @@ template <int DT, int D, bool WIDE>
 struct AttnShape {
   static constexpr int kElem = DT == D3_DTYPE_E4M3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  // keys of one warp and stage: about 8 KB of keys and as much of values
-  static constexpr int kNK = 8192 / kRowBytes < 64 ? 8192 / kRowBytes : 64;
+  // keys of one warp and tile: a slot of the ring holds up to 8 KB
+  static constexpr int kNK = 8192 / kRowBytes < 32 ? 8192 / kRowBytes : 32;
   static constexpr int kTile = kNK * kAttnWarps;
   static constexpr int kRows = WIDE ? 16 : 8;
-  static constexpr int kHalf = kNK * kRowBytes;  // bytes of a stage's keys
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int kJoin = kAttnWarps * kRows * D * 4;  // the warps' output rows
-  static constexpr int kRing = kAttnWarps * kStage;
-  static constexpr int kStages = 3 * kRing + kJoin + 2048 <= 227 * 1024 ? 3 : 2;
-  static constexpr int kSmem = kStages * kRing + kJoin + 2048;
+  static constexpr int kHalf = kNK * kRowBytes;  // bytes of a slot
+  static constexpr int kAhead = (24576 / kHalf - 1) / 2 < 4 ? (24576 / kHalf - 1) / 2 : 4;  // tiles loaded ahead
+  static constexpr int kSlots = 2 * kAhead + 1;
+  static constexpr int kWarpRing = kSlots * kHalf;
+  static constexpr int kRing = kAttnWarps * kWarpRing;
+  // output rows of kJoinWarps warps at a time are added up in shared memory
+  static constexpr int kJoinWarps = 32768 / (kRows * D * 4) < kAttnWarps ? 32768 / (kRows * D * 4) : kAttnWarps;
+  static constexpr int kJoin = kJoinWarps * kRows * D * 4;
+  static constexpr int kSmem = kRing + kJoin + 2048;
   static constexpr int kRecord = kRows * (D + 2);  // floats of a partial result
 };
 
@@ -146,15 +149,15 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs& a, int b) {
 }
 
 // Tiles of one CTA: an equal share of the line, at least kMinShare.
-constexpr int kMinShare = 2;
+constexpr int kMinShare = 1;
 __device__ __forceinline__ int64_t cta_share(int64_t total, int grid) {
   const int64_t s = (total + grid - 1) / grid;
   return s < kMinShare ? kMinShare : s;
 }
 
-// Sums over the sequences with 128 threads: the tiles of all units of all
+// Sums over the sequences with all threads: the tiles of all units of all
 // sequences, and each thread's exclusive prefix over its own run of `per`
-// sequences. scratch: 8 values of shared memory.
+// sequences. scratch: kAttnWarps values of shared memory.
 template <int TILE>
 __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int64_t* scratch, int64_t& mine,
                                           int64_t& before, int64_t& total) {
@@ -209,12 +212,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   constexpr bool BF16 = DT == D3_DTYPE_BF16;        // type of the matrix products
   constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
   constexpr bool SPLIT = BF16 && !WIDE;             // rows 8-15 carry the rounding's rest
-  constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kStages, ROWS = Sh::kRows;
+  constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kSlots, P = Sh::kAhead, ROWS = Sh::kRows;
   constexpr int KS = D / 16, NT = NK / 8, DT8 = D / 8;
-  constexpr int PIECES = RB / 16, RPL = (NK + 31) / 32;  // rows whose page a lane looks up
+  constexpr int PIECES = RB / 16, JW = Sh::kJoinWarps;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* join = reinterpret_cast<float*>(smem + S * Sh::kRing);
-  float* stat = reinterpret_cast<float*>(smem + S * Sh::kRing + Sh::kJoin);  // [warps][2][16]
+  float* join = reinterpret_cast<float*>(smem + Sh::kRing);
+  float* stat = reinterpret_cast<float*>(smem + Sh::kRing + Sh::kJoin);  // [warps][2][16]
   int64_t* scratch = reinterpret_cast<int64_t*>(stat + kAttnWarps * 32);
   int* start = reinterpret_cast<int*>(scratch + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -254,73 +257,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   cur.enter(a);
   Cursor<Sh::kTile> ld = cur;
 
-  const uint32_t ring = smem_u32(smem) + warp * Sh::kStage;  // + stage * kRing
+  const uint32_t ring = smem_u32(smem) + warp * Sh::kWarpRing;
 
-  // pages of the rows of tile `ld` that this lane looks up (row = lane + 32 i)
-  int page[RPL], off[RPL];
+  // offsets of row `lane` of tile `ld` in the two caches (-1: past the end)
+  int64_t koff, voff;
   auto look_up = [&]() {
-#pragma unroll
-    for (int i = 0; i < RPL; ++i) {
-      const int j = ld.begin + ld.tile * Sh::kTile + warp * NK + lane + 32 * i;
-      page[i] = -1;
-      if (lane + 32 * i < NK && j < ld.len) {
-        const int slot = j / a.page_size;
-        off[i] = j - slot * a.page_size;
-        int p = __ldg(a.table + ld.b * a.table_stride + slot);
-        if (p < 0 || p >= a.num_pages) {
-          if (a.status) atomicExch(a.status, kDevBadRow);
-          p = 0;
-        }
-        page[i] = p;
+    const int j = ld.begin + ld.tile * Sh::kTile + warp * NK + lane;
+    koff = voff = -1;
+    if (lane < NK && j < ld.len) {
+      const int slot = j / a.page_size;
+      const int64_t o = j - slot * a.page_size;
+      int p = __ldg(a.table + ld.b * a.table_stride + slot);
+      if (p < 0 || p >= a.num_pages) {
+        if (a.status) atomicExch(a.status, kDevBadRow);
+        p = 0;
       }
+      koff = p * a.k_page + o * a.k_token;
+      voff = p * a.v_page + o * a.v_token;
     }
   };
-  // copies this warp's rows of tile `ld` into stage s; rows past the sequence's
-  // end are zeroed (what the cache holds there may be anything, NaN included)
-  auto load = [&](int s) {
-    const int head = ld.unit / a.parts;
-    const uint8_t* kb = a.k + head * a.k_head;
-    const uint8_t* vb = a.v + head * a.v_head;
-    const uint32_t dst = ring + s * Sh::kRing;
+  // copies this warp's rows of tile `ld` (keys or values) into a slot; rows past
+  // the sequence's end are zeroed (what the cache holds there may be anything,
+  // NaN included)
+  auto load = [&](int slot, const uint8_t* base, int64_t mine_off) {
+    const uint32_t dst = ring + slot * Sh::kHalf;
 #pragma unroll
     for (int it = 0; it < NK * PIECES / 32; ++it) {
       const int idx = it * 32 + lane, r = idx / PIECES, c = idx % PIECES;
-      const int from = (it * 32 / PIECES) >> 5;  // which of the lanes' rows (uniform)
-      int p, o;
-      if constexpr (RPL == 1) {
-        p = __shfl_sync(0xffffffffu, page[0], r);
-        o = __shfl_sync(0xffffffffu, off[0], r);
-      } else {
-        p = __shfl_sync(0xffffffffu, page[from], r & 31);
-        o = __shfl_sync(0xffffffffu, off[from], r & 31);
-      }
-      const bool take = p >= 0;
-      const int64_t pp = take ? p : 0, oo = take ? o : 0;
-      const uint32_t at = ring_at<RB>(r, c);
-      cp_async_16_zfill(dst + at, kb + pp * a.k_page + oo * a.k_token + c * 16, take);
-      cp_async_16_zfill(dst + Sh::kHalf + at, vb + pp * a.v_page + oo * a.v_token + c * 16, take);
+      const int64_t o = __shfl_sync(0xffffffffu, mine_off, r);
+      cp_async_16_zfill(dst + ring_at<RB>(r, c), base + (o < 0 ? 0 : o) + c * 16, o >= 0);
     }
   };
-
-  int loaded = 0;
-  look_up();
-#pragma unroll
-  for (int s = 0; s < S - 1; ++s) {
+  int loaded = 0;  // tiles whose values have been asked for
+  int slot = 0;    // next slot to fill
+  auto load_keys = [&]() {
+    if (loaded < count) load(slot, a.k + ld.unit / a.parts * a.k_head, koff);
+    slot = slot + 1 == S ? 0 : slot + 1;
+    cp_async_commit();
+  };
+  auto load_values = [&]() {
     if (loaded < count) {
-      load(s);
+      load(slot, a.v + ld.unit / a.parts * a.v_head, voff);
       if (++loaded < count) {
         ld.next(a);
         look_up();
       }
     }
+    slot = slot + 1 == S ? 0 : slot + 1;
     cp_async_commit();
+  };
+
+  look_up();
+#pragma unroll
+  for (int s = 0; s < P; ++s) {
+    load_keys();
+    load_values();
   }
 
   uint32_t qf[KS][WIDE ? 4 : 2];
   float o[DT8][4], m[WIDE ? 2 : 1], l[WIDE ? 2 : 1];
   float lg[WIDE ? 2 : 1];  // logit in units of log2 per product
   bool opened = false, whole = false;
-  int seg_slot = 0;
+  int seg_slot = 0, use = 0;
   for (int i = 0; i < count; ++i) {
     const int head = cur.unit / a.parts;
     const int h0 = head * a.group + (cur.unit % a.parts) * ROWS;
@@ -373,19 +371,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         lg[w] = ks;
       }
     }
-    // the next stage's loads go out before this stage's work
-    if (loaded < count) {
-      load((i + S - 1) % S);
-      if (++loaded < count) {
-        ld.next(a);
-        look_up();
-      }
-    }
-    cp_async_commit();
+    // the next loads go out before this tile's work
+    load_keys();
     cp_async_wait<S - 1>();
     __syncwarp();
-
-    const uint32_t ks = ring + (i % S) * Sh::kRing, vs = ks + Sh::kHalf;
+    const uint32_t ks = ring + use * Sh::kHalf;
+    use = use + 1 == S ? 0 : use + 1;
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -469,6 +460,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
       }
     }
     // out += P V
+    __syncwarp();  // every lane has read the keys' slot: it may be filled again
+    load_values();
+    cp_async_wait<S - 1>();
+    __syncwarp();
+    const uint32_t vs = ring + use * Sh::kHalf;
+    use = use + 1 == S ? 0 : use + 1;
     if constexpr (DT == D3_DTYPE_E4M3) {
 #pragma unroll
       for (int n = 0; n < NT; n += 2)
@@ -500,7 +497,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           mma_16816<BF16>(o[c + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[2], b[3]);
         }
     }
-    __syncwarp();  // every lane has read this stage before it is loaded again
+    __syncwarp();  // the same for the values
 
     const bool last = cur.tile + 1 == cur.tiles;
     if (last || i + 1 == count) {
@@ -514,23 +511,43 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           stat[warp * 32 + quad + 8 * w] = m[w];
           stat[warp * 32 + 16 + quad + 8 * w] = l[w];
         }
-        float* row = join + (warp * ROWS + quad + 8 * w) * D;
-#pragma unroll
-        for (int d = 0; d < DT8; ++d) {
-          float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
-          if constexpr (SPLIT) {
-            x0 += o[d][2];
-            x1 += o[d][3];
-          }
-          if constexpr (DT == D3_DTYPE_E4M3) {
-            row[(d >> 1) * 16 + 4 * t4 + (d & 1)] = x0;
-            row[(d >> 1) * 16 + 4 * t4 + 2 + (d & 1)] = x1;
-          } else {
-            *reinterpret_cast<float2*>(row + d * 8 + 2 * t4) = make_float2(x0, x1);
-          }
-        }
       }
       __syncthreads();
+      // each warp scales its rows to the common maximum; JW at a time they are
+      // added into JW buffers, in the order of the warps
+#pragma unroll 1
+      for (int round = 0; round < kAttnWarps / JW; ++round) {
+        if (warp / JW == round) {
+#pragma unroll
+          for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, stat[x * 32 + quad + 8 * w]);
+            const float f = exp2f(m[w] - (top == -INFINITY ? 0.f : top));
+            float* row = join + ((warp % JW) * ROWS + quad + 8 * w) * D;
+#pragma unroll
+            for (int d = 0; d < DT8; ++d) {
+              float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
+              if constexpr (SPLIT) {
+                x0 += o[d][2];
+                x1 += o[d][3];
+              }
+              x0 *= f;
+              x1 *= f;
+              if constexpr (DT == D3_DTYPE_E4M3) {
+                float* at = row + (d >> 1) * 16 + 4 * t4 + (d & 1);
+                at[0] = round ? at[0] + x0 : x0;
+                at[2] = round ? at[2] + x1 : x1;
+              } else {
+                float2* at = reinterpret_cast<float2*>(row + d * 8 + 2 * t4);
+                const float2 was = round ? *at : make_float2(0.f, 0.f);
+                *at = make_float2(was.x + x0, was.y + x1);
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
       whole = whole && last;
       float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
       const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
@@ -543,14 +560,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         const float base = top == -INFINITY ? 0.f : top;
         float sum = 0.f, x[4] = {};
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) {
-          const float f = exp2f(stat[w * 32 + r] - base);
-          sum += f * stat[w * 32 + 16 + r];
+        for (int w = 0; w < kAttnWarps; ++w)
+          sum += exp2f(stat[w * 32 + r] - base) * stat[w * 32 + 16 + r];
+#pragma unroll
+        for (int w = 0; w < JW; ++w) {
           const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * D + d);
-          x[0] = fmaf(f, y.x, x[0]);
-          x[1] = fmaf(f, y.y, x[1]);
-          x[2] = fmaf(f, y.z, x[2]);
-          x[3] = fmaf(f, y.w, x[3]);
+          x[0] += y.x;
+          x[1] += y.y;
+          x[2] += y.z;
+          x[3] += y.w;
         }
         if (whole) {
           const float inv = sum == 0.f ? 0.f : vsc / sum;  // a NaN stays one
