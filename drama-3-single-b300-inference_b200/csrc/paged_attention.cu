@@ -73,10 +73,17 @@ struct AttnShape {
   static constexpr int kSlots = 2 * kAhead + 1;
   static constexpr int kWarpRing = kSlots * kHalf;
   static constexpr int kRing = kAttnWarps * kWarpRing;
+  static constexpr int kQPitch = D * 2 + 16;   // bytes of a query row, padded against bank conflicts
+  static constexpr int kQ = kRows * kQPitch;
+  static constexpr int kQPieces = (kRows * D * 2 / 16 + kAttnThreads - 1) / kAttnThreads;  // of one thread
   // output rows of kJoinWarps warps at a time are added up in shared memory
-  static constexpr int kJoinWarps = 32768 / (kRows * D * 4) < kAttnWarps ? 32768 / (kRows * D * 4) : kAttnWarps;
-  static constexpr int kJoin = kJoinWarps * kRows * D * 4;
-  static constexpr int kSmem = kRing + kJoin + 2048;
+  static constexpr int kJoinPitch = D + (kElem == 1 ? 16 : 8);  // floats, padded likewise
+  static constexpr int kJoinFit = 20480 / (kRows * kJoinPitch * 4);
+  static constexpr int kJoinWarps = kJoinFit >= 8 ? 8 : kJoinFit >= 4 ? 4 : kJoinFit >= 2 ? 2 : 1;
+  static constexpr int kJoin = kJoinWarps * kRows * kJoinPitch * 4;
+  static constexpr int kStat = kAttnWarps * 32 * 4 + 64;
+  static constexpr int kSmem = kRing + kJoin + kQ + kStat;
+  static_assert(kSmem <= 227 * 1024);
   static constexpr int kRecord = kRows * (D + 2);  // floats of a partial result
 };
 
@@ -150,17 +157,16 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs& a, int b) {
 
 // Tiles of one CTA: an equal share of the line, at least kMinShare.
 constexpr int kMinShare = 1;
-__device__ __forceinline__ int64_t cta_share(int64_t total, int grid) {
-  const int64_t s = (total + grid - 1) / grid;
-  return s < kMinShare ? kMinShare : s;
+__device__ __forceinline__ int cta_share(int total, int grid) {
+  return max(kMinShare, static_cast<int>((static_cast<unsigned>(total) + grid - 1) / grid));
 }
 
 // Sums over the sequences with all threads: the tiles of all units of all
 // sequences, and each thread's exclusive prefix over its own run of `per`
 // sequences. scratch: kAttnWarps values of shared memory.
 template <int TILE>
-__device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int64_t* scratch, int64_t& mine,
-                                          int64_t& before, int64_t& total) {
+__device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int* scratch, int& mine, int& before,
+                                          int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   mine = 0;
   for (int i = 0; i < per; ++i) {
@@ -168,10 +174,10 @@ __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int64_t* s
     if (b < a.B) mine += seq_tiles<TILE>(a, b);
   }
   mine *= a.units;
-  int64_t x = mine;
+  int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) scratch[warp] = x;
@@ -206,6 +212,18 @@ struct Cursor {
   }
 };
 
+// Four columns of a finished row: x / sum * v_scale in the output's type; lse
+// with the first. A sum of 0 (no key took part) gives zeros and -inf, a NaN stays one.
+template <bool BF16>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int d, const float (&x)[4], float sum,
+                                          float top, float v_scale) {
+  const float inv = sum == 0.f ? 0.f : v_scale / sum;
+  *reinterpret_cast<uint2*>(a.out + b * a.out_row + h * a.out_head + d) =
+      make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+  if (a.lse && d == 0)
+    a.lse[static_cast<int64_t>(b) * a.q_heads + h] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
+}
+
 template <int DT, int D, bool WIDE>
 __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
@@ -214,12 +232,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   constexpr bool SPLIT = BF16 && !WIDE;             // rows 8-15 carry the rounding's rest
   constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kSlots, P = Sh::kAhead, ROWS = Sh::kRows;
   constexpr int KS = D / 16, NT = NK / 8, DT8 = D / 8;
-  constexpr int PIECES = RB / 16, JW = Sh::kJoinWarps;
+  constexpr int PIECES = RB / 16, JW = Sh::kJoinWarps, JP = Sh::kJoinPitch;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* join = reinterpret_cast<float*>(smem + Sh::kRing);
-  float* stat = reinterpret_cast<float*>(smem + Sh::kRing + Sh::kJoin);  // [warps][2][16]
-  int64_t* scratch = reinterpret_cast<int64_t*>(stat + kAttnWarps * 32);
-  int* start = reinterpret_cast<int*>(scratch + 8);
+  uint8_t* qs = smem + Sh::kRing + Sh::kJoin;
+  float* stat = reinterpret_cast<float*>(qs + Sh::kQ);  // [warps][2][16]
+  int* scratch = reinterpret_cast<int*>(stat + kAttnWarps * 32);
+  int* start = scratch + kAttnWarps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int quad = lane >> 2, t4 = lane & 3;
 
@@ -228,25 +247,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
 
   // where this CTA's share of the line begins
   const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
-  int64_t mine, before, total;
+  int mine, before, total;
   line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
-  const int64_t share = cta_share(total, a.grid);
-  const int64_t first = blockIdx.x * share;
-  if (first >= total) return;
-  const int count = static_cast<int>(min(share, total - first));
+  const int share = cta_share(total, a.grid);
+  if (blockIdx.x > static_cast<unsigned>((total - 1) / share) || total == 0) return;
+  const int first = blockIdx.x * share;
+  const int count = min(share, total - first);
   if (first >= before && first < before + mine) {
-    int64_t at = before;
+    int at = before;
     for (int i = 0; i < per; ++i) {
       const int b = tid * per + i;
-      const int64_t n = static_cast<int64_t>(seq_tiles<Sh::kTile>(a, b)) * a.units;
-      if (first < at + n) {
-        const int tiles = static_cast<int>(n / a.units);
+      const int tiles = seq_tiles<Sh::kTile>(a, b);
+      if (first < at + tiles * a.units) {
         start[0] = b;
-        start[1] = static_cast<int>((first - at) / tiles);
-        start[2] = static_cast<int>((first - at) % tiles);
+        start[1] = (first - at) / tiles;
+        start[2] = (first - at) % tiles;
         break;
       }
-      at += n;
+      at += tiles * a.units;
     }
   }
   __syncthreads();
@@ -307,12 +325,35 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     cp_async_commit();
   };
 
+  // queries of a unit, on their way to shared memory (rows past the unit's are zero)
+  uint4 qreg[Sh::kQPieces];
+  auto fetch_q = [&](const Cursor<Sh::kTile>& c) {
+    const int head = c.unit / a.parts, h0 = head * a.group + (c.unit % a.parts) * ROWS;
+    const int nh = min(ROWS, (head + 1) * a.group - h0);
+#pragma unroll
+    for (int x = 0; x < Sh::kQPieces; ++x) {
+      const int e = tid + x * kAttnThreads, r = e / (D / 8), d = e % (D / 8) * 8;
+      qreg[x] = r < nh ? __ldg(reinterpret_cast<const uint4*>(a.q + c.b * a.q_row + (h0 + r) * a.q_head + d)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto place_q = [&]() {
+#pragma unroll
+    for (int x = 0; x < Sh::kQPieces; ++x) {
+      const int e = tid + x * kAttnThreads, r = e / (D / 8), d = e % (D / 8) * 16;
+      if (r < ROWS) *reinterpret_cast<uint4*>(qs + r * Sh::kQPitch + d) = qreg[x];
+    }
+  };
+
+  fetch_q(cur);
   look_up();
 #pragma unroll
   for (int s = 0; s < P; ++s) {
     load_keys();
     load_values();
   }
+
+  place_q();
+  __syncthreads();
 
   uint32_t qf[KS][WIDE ? 4 : 2];
   float o[DT8][4], m[WIDE ? 2 : 1], l[WIDE ? 2 : 1];
@@ -335,38 +376,36 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
       for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
         m[w] = -INFINITY;
         l[w] = 0.f;
-        const int r = quad + 8 * w;
-        const uint16_t* row = a.q + cur.b * a.q_row + static_cast<int64_t>(h0 + (r < nh ? r : 0)) * a.q_head;
+        const uint8_t* row = qs + (quad + 8 * w) * Sh::kQPitch;
         float ks = a.scale * kLog2e;
         if constexpr (DT == D3_DTYPE_E4M3) {
           // the row's largest element decides its power of two
           float top = 0.f;
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) top = fmaxf(top, fabsf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + x))));
+          for (int s = 0; s < KS; ++s) {
+            const uint2 x = *reinterpret_cast<const uint2*>(row + 32 * s + 8 * t4);
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x.x << 16)), fabsf(__uint_as_float(x.x & 0xffff0000u))));
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x.y << 16)), fabsf(__uint_as_float(x.y & 0xffff0000u))));
+          }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           int e = 0;
           if (top > 0.f && isfinite(top)) frexpf(top, &e);
+          e = max(-100, min(100, e));  // 2^-e and 2^e both exist
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const float lo = ldexpf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + 2 * x)), -e);
-              const float hi = ldexpf(bf16_bits_to_f32(__ldg(row + 16 * s + 4 * t4 + 2 * x + 1)), -e);
-              qf[s][WIDE ? 2 * x + w : x] = r < nh ? pack16<false>(lo, hi) : 0u;
-            }
-          ks = ldexpf(ks * (a.k_scale ? __ldg(a.k_scale + head) : 1.0f), e);
+          for (int s = 0; s < KS; ++s) {
+            const uint2 y = *reinterpret_cast<const uint2*>(row + 32 * s + 8 * t4);
+            qf[s][w] = pack16<false>(__uint_as_float(y.x << 16) * down, __uint_as_float(y.x & 0xffff0000u) * down);
+            qf[s][WIDE ? 2 + w : 1] = pack16<false>(__uint_as_float(y.y << 16) * down, __uint_as_float(y.y & 0xffff0000u) * down);
+          }
+          ks *= (a.k_scale ? __ldg(a.k_scale + head) : 1.0f) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         } else {
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint16_t* p = row + 16 * s + 2 * t4 + 8 * x;
-              const uint32_t two = static_cast<uint32_t>(__ldg(p)) | (static_cast<uint32_t>(__ldg(p + 1)) << 16);
-              qf[s][WIDE ? 2 * x + w : x] = r < nh ? two : 0u;
-            }
+          for (int s = 0; s < KS; ++s) {
+            qf[s][w] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4);
+            qf[s][WIDE ? 2 + w : 1] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4 + 16);
+          }
         }
         lg[w] = ks;
       }
@@ -503,6 +542,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     if (last || i + 1 == count) {
       // join the warps: (max, sum) and output rows through shared memory
       opened = false;
+      const bool more = i + 1 < count;
+      Cursor<Sh::kTile> nxt = cur;
+      if (more) {
+        nxt.next(a);
+        fetch_q(nxt);
+      }
 #pragma unroll
       for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
         l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
@@ -524,24 +569,26 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
 #pragma unroll
             for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, stat[x * 32 + quad + 8 * w]);
             const float f = exp2f(m[w] - (top == -INFINITY ? 0.f : top));
-            float* row = join + ((warp % JW) * ROWS + quad + 8 * w) * D;
+            float* row = join + ((warp % JW) * ROWS + quad + 8 * w) * JP;
+            if constexpr (DT == D3_DTYPE_E4M3) {
 #pragma unroll
-            for (int d = 0; d < DT8; ++d) {
-              float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
-              if constexpr (SPLIT) {
-                x0 += o[d][2];
-                x1 += o[d][3];
+              for (int d = 0; d < DT8; d += 2) {
+                float4* at = reinterpret_cast<float4*>(row + d * 8 + 4 * t4);
+                const float4 was = round ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                *at = make_float4(fmaf(o[d][2 * w], f, was.x), fmaf(o[d + 1][2 * w], f, was.y),
+                                  fmaf(o[d][2 * w + 1], f, was.z), fmaf(o[d + 1][2 * w + 1], f, was.w));
               }
-              x0 *= f;
-              x1 *= f;
-              if constexpr (DT == D3_DTYPE_E4M3) {
-                float* at = row + (d >> 1) * 16 + 4 * t4 + (d & 1);
-                at[0] = round ? at[0] + x0 : x0;
-                at[2] = round ? at[2] + x1 : x1;
-              } else {
+            } else {
+#pragma unroll
+              for (int d = 0; d < DT8; ++d) {
+                float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
+                if constexpr (SPLIT) {
+                  x0 += o[d][2];
+                  x1 += o[d][3];
+                }
                 float2* at = reinterpret_cast<float2*>(row + d * 8 + 2 * t4);
                 const float2 was = round ? *at : make_float2(0.f, 0.f);
-                *at = make_float2(was.x + x0, was.y + x1);
+                *at = make_float2(fmaf(x0, f, was.x), fmaf(x1, f, was.y));
               }
             }
           }
@@ -564,22 +611,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           sum += exp2f(stat[w * 32 + r] - base) * stat[w * 32 + 16 + r];
 #pragma unroll
         for (int w = 0; w < JW; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * D + d);
+          const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * JP + d);
           x[0] += y.x;
           x[1] += y.y;
           x[2] += y.z;
           x[3] += y.w;
         }
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : vsc / sum;  // a NaN stays one
-          const uint2 two = make_uint2(pack16<QBF16>(x[0] * inv, x[1] * inv), pack16<QBF16>(x[2] * inv, x[3] * inv));
-          uint16_t* at = a.out + cur.b * a.out_row + (h0 + r) * a.out_head + d;
-          at[0] = static_cast<uint16_t>(two.x);
-          at[1] = static_cast<uint16_t>(two.x >> 16);
-          at[2] = static_cast<uint16_t>(two.y);
-          at[3] = static_cast<uint16_t>(two.y >> 16);
-          if (a.lse && d == 0)
-            a.lse[static_cast<int64_t>(cur.b) * a.q_heads + h0 + r] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
+          store_row<QBF16>(a, cur.b, h0 + r, d, x, sum, top, vsc);
         } else {
           *reinterpret_cast<float4*>(rec + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
           if (d == 0) {
@@ -588,73 +627,104 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
           }
         }
       }
+      if (more) place_q();  // every warp took its queries before the barriers above
+      cur = nxt;
       __syncthreads();
+    } else {
+      ++cur.tile;
     }
-    if (i + 1 < count) cur.next(a);
   }
   cp_async_wait<0>();
 }
 
-// One CTA per unit: units without keys get zeros, units that several CTAs
-// shared are joined from their records in CTA order.
+// One CTA per query row: rows without keys get zeros, rows of units that several
+// CTAs shared are joined from their records. Groups of D / 4 threads add up every
+// (256 * 4 / D)-th record, so the loads of a long unit's records overlap; the
+// groups are then added in order.
 template <int DT, int D, bool WIDE>
 __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool QBF16 = DT != D3_DTYPE_F16;
-  constexpr int ROWS = Sh::kRows;
-  __shared__ int64_t scratch[8], found;
-  const int tid = threadIdx.x;
-  const int b = blockIdx.x / a.units, unit = blockIdx.x % a.units;
+  constexpr int ROWS = Sh::kRows, LANES = D / 4, GROUPS = kAttnThreads / LANES;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float4* acc = reinterpret_cast<float4*>(smem);                       // [GROUPS][LANES]
+  float* fac = reinterpret_cast<float*>(smem) + kAttnThreads * 4;      // [a.grid] maximum, then weight
+  float* red = fac + a.grid;                                           // [2][warps]
+  int* scratch = reinterpret_cast<int*>(red + 2 * kAttnWarps);
+  int* found = scratch + kAttnWarps;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads;
+  const int head = h / a.group, part = (h - head * a.group) / ROWS, r = (h - head * a.group) % ROWS;
+  const int unit = head * a.parts + part;
   const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
   pdl_trigger();
-  int64_t mine, before, total;
+  int mine, before, total;
   line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
   const int tiles = seq_tiles<Sh::kTile>(a, b);
   if (b / per == tid) {
-    int64_t at = before;
-    for (int x = tid * per; x < b; ++x) at += static_cast<int64_t>(seq_tiles<Sh::kTile>(a, x)) * a.units;
-    found = at + static_cast<int64_t>(unit) * tiles;
+    int at = before;
+    for (int x = tid * per; x < b; ++x) at += seq_tiles<Sh::kTile>(a, x) * a.units;
+    *found = at + unit * tiles;
   }
   __syncthreads();
-  const int64_t share = cta_share(total, a.grid);
-  const int64_t lo = found, hi = lo + tiles;  // the unit's tiles on the line
-  const int c0 = static_cast<int>(lo / share), c1 = static_cast<int>((hi - 1) / share);
+  const int share = cta_share(total, a.grid);
+  const int lo = *found, hi = lo + tiles;  // the unit's tiles on the line
+  const int c0 = lo / share, n = tiles > 0 ? (hi - 1) / share - c0 + 1 : 0;
   // every CTA waits: a kernel after this one waits for this grid only, which
   // must not be complete before the main kernel is
   pdl_wait();
-  if (tiles > 0 && c0 == c1) return;
-  const int head = unit / a.parts;
-  const int h0 = head * a.group + (unit % a.parts) * ROWS;
-  const int nh = min(ROWS, (head + 1) * a.group - h0);
-  const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
-  for (int e = tid * 4; e < nh * D; e += kAttnThreads * 4) {
-    const int r = e / D, d = e % D;
-    float top = -INFINITY, sum = 0.f, x[4] = {};
-    if (tiles > 0) {
-      for (int c = c0; c <= c1; ++c) {
-        const float* rec = a.partial + (static_cast<int64_t>(c) * 2 + (c == c0 && lo % share != 0)) * Sh::kRecord;
-        const float mc = __ldcg(rec + ROWS * D + r), lc = __ldcg(rec + ROWS * D + ROWS + r);
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(rec + r * D + d));
-        const float mn = fmaxf(top, mc), base = mn == -INFINITY ? 0.f : mn;
-        const float f = exp2f(top - base), g = exp2f(mc - base);
-        top = mn;
-        sum = sum * f + lc * g;
-        x[0] = x[0] * f + y.x * g;
-        x[1] = x[1] * f + y.y * g;
-        x[2] = x[2] * f + y.z * g;
-        x[3] = x[3] * f + y.w * g;
-      }
-    }
-    const float inv = sum == 0.f ? 0.f : vsc / sum;
-    const uint2 two = make_uint2(pack16<QBF16>(x[0] * inv, x[1] * inv), pack16<QBF16>(x[2] * inv, x[3] * inv));
-    uint16_t* at = a.out + b * a.out_row + (h0 + r) * a.out_head + d;
-    at[0] = static_cast<uint16_t>(two.x);
-    at[1] = static_cast<uint16_t>(two.x >> 16);
-    at[2] = static_cast<uint16_t>(two.y);
-    at[3] = static_cast<uint16_t>(two.y >> 16);
-    if (a.lse && d == 0)
-      a.lse[static_cast<int64_t>(b) * a.q_heads + h0 + r] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
+  if (n == 1) return;
+  // the first record lies in its CTA's second place where the CTA began with another unit
+  const float* rec0 = a.partial + (static_cast<int64_t>(c0) * 2 + (lo != c0 * share)) * Sh::kRecord;
+  const float* rec = a.partial + static_cast<int64_t>(c0) * 2 * Sh::kRecord;  // + 2 c records, c > 0
+  auto record = [&](int c) { return c == 0 ? rec0 : rec + static_cast<int64_t>(c) * 2 * Sh::kRecord; };
+  float top = -INFINITY, sum = 0.f;
+  for (int c = tid; c < n; c += kAttnThreads) {
+    const float m = __ldcg(record(c) + ROWS * D + r);
+    fac[c] = m;
+    top = fmaxf(top, m);
   }
+  top = warp_max(top);
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, red[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int c = tid; c < n; c += kAttnThreads) {
+    const float f = exp2f(fac[c] - base);
+    fac[c] = f;
+    sum += f * __ldcg(record(c) + ROWS * D + ROWS + r);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[kAttnWarps + warp] = sum;
+  __syncthreads();
+  const int d = tid % LANES, g = tid / LANES;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = g; c < n; c += GROUPS) {
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(record(c) + r * D) + d);
+    const float f = fac[c];
+    x.x = fmaf(f, y.x, x.x);
+    x.y = fmaf(f, y.y, x.y);
+    x.z = fmaf(f, y.z, x.z);
+    x.w = fmaf(f, y.w, x.w);
+  }
+  acc[g * LANES + d] = x;
+  __syncthreads();
+  if (g != 0) return;
+  float out[4] = {};
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kAttnWarps; ++w) sum += red[kAttnWarps + w];
+  for (int i = 0; i < GROUPS; ++i) {
+    const float4 y = acc[i * LANES + d];
+    out[0] += y.x;
+    out[1] += y.y;
+    out[2] += y.z;
+    out[3] += y.w;
+  }
+  store_row<QBF16>(a, b, h, d * 4, out, sum, top, a.v_scale ? __ldg(a.v_scale + head) : 1.0f);
 }
 
 template <int DT, int D, bool WIDE>
@@ -669,7 +739,8 @@ int launch_attention(AttnArgs& a, cudaStream_t s) {
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   launch_kernel(paged_attention_kernel<DT, D, WIDE>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
-  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.units)), dim3(kAttnThreads), 0, s, a);
+  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.q_heads)), dim3(kAttnThreads),
+                kAttnThreads * 16 + (a.grid + 3 * kAttnWarps + 1) * 4, s, a);
   return check_launch("d3_paged_attention");
 }
 
@@ -751,7 +822,12 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   a.partial = static_cast<float*>(workspace);
   a.grid = sm_count();
   a.status = status;
-  D3_REQUIRE(static_cast<int64_t>(B) * a.units <= 0x7fffffff, "batch or heads too large");
+  D3_REQUIRE(aligned(q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0, "rows of q must be 16-byte aligned");
+  D3_REQUIRE(aligned(out, 8) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0, "rows of out must be 8-byte aligned");
+  // the line of tiles (64 keys at least, see AttnShape) is counted in 32 bits
+  D3_REQUIRE(static_cast<int64_t>(B) * a.units * (a.max_len / 64 + 1) < 0x40000000 &&
+                 static_cast<int64_t>(B) * q_heads <= 0x7fffffff,
+             "batch, heads and length are too large for one call");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int D = cache->dim;
   switch (cache->dtype) {
