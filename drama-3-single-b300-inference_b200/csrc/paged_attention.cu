@@ -7,14 +7,14 @@
 // hide behind the loads.
 //
 // Work. A unit is a (sequence, key head, group of query heads); its keys are
-// cut into tiles of 8 * NK. All units' tiles form one line, and each CTA of a
-// persistent grid (one per SM) takes an equal share of it, so ragged lengths
+// cut into tiles of 4 * NK. All units' tiles form one line, and each CTA of a
+// persistent grid (two per SM) takes an equal share of it, so ragged lengths
 // balance by themselves and a single long sequence uses every SM. A CTA's share
 // may end inside a unit: such parts leave (max, sum, output row) in the
 // workspace, and a second kernel joins them in CTA order (no atomics, so equal
 // inputs give equal bits).
 //
-// Inside a CTA 8 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
+// Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
 // tile, loads them with cp.async into its own ring of shared-memory slots (keys
 // and values of a tile are two slots; no barrier between warps), and works with mma.sync m16n8k16: queries are
 // the 16 rows of A, keys the columns of B for the logits, and the probabilities
@@ -32,8 +32,9 @@
 namespace d3 {
 namespace {
 
-constexpr int kAttnWarps = 8;
+constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kMaxSmem = 113 * 1024;  // of one CTA: two share an SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -76,14 +77,14 @@ struct AttnShape {
   static constexpr int kQPitch = D * 2 + 16;   // bytes of a query row, padded against bank conflicts
   static constexpr int kQ = kRows * kQPitch;
   static constexpr int kQPieces = (kRows * D * 2 / 16 + kAttnThreads - 1) / kAttnThreads;  // of one thread
-  // output rows of kJoinWarps warps at a time are added up in shared memory
-  static constexpr int kJoinPitch = D + (kElem == 1 ? 16 : 8);  // floats, padded likewise
-  static constexpr int kJoinFit = 20480 / (kRows * kJoinPitch * 4);
-  static constexpr int kJoinWarps = kJoinFit >= 8 ? 8 : kJoinFit >= 4 ? 4 : kJoinFit >= 2 ? 2 : 1;
-  static constexpr int kJoin = kJoinWarps * kRows * kJoinPitch * 4;
   static constexpr int kStat = kAttnWarps * 32 * 4 + 64;
+  // 8 output rows of kJoinWarps warps at a time are added up in shared memory
+  static constexpr int kJoinPitch = D + (D == 256 && WIDE ? 4 : kElem == 1 ? 16 : 8);  // floats, padded likewise
+  static constexpr int kJoinFit = (kMaxSmem - kRing - kQ - kStat) / (8 * kJoinPitch * 4);
+  static constexpr int kJoinWarps = kJoinFit >= 4 ? 4 : kJoinFit >= 2 ? 2 : 1;
+  static constexpr int kJoin = kJoinWarps * 8 * kJoinPitch * 4;
   static constexpr int kSmem = kRing + kJoin + kQ + kStat;
-  static_assert(kSmem <= 227 * 1024);
+  static_assert(kSmem <= kMaxSmem);
   static constexpr int kRecord = kRows * (D + 2);  // floats of a partial result
 };
 
@@ -155,13 +156,22 @@ __device__ __forceinline__ int seq_tiles(const AttnArgs& a, int b) {
   return (len - seq_begin(a, len) + TILE - 1) / TILE;
 }
 
-// Tiles of one CTA: an equal share of the line, at least kMinShare.
-constexpr int kMinShare = 1;
-__device__ __forceinline__ int cta_share(int total, int grid) {
-  return max(kMinShare, static_cast<int>((static_cast<unsigned>(total) + grid - 1) / grid));
+// Places on the line: a unit with keys takes kUnitCost places of its own before
+// its tiles, for what a unit costs besides them (fetching its queries and page
+// numbers, joining the warps).
+constexpr int kUnitCost = 1;
+template <int TILE>
+__device__ __forceinline__ int seq_places(const AttnArgs& a, int b) {
+  const int tiles = seq_tiles<TILE>(a, b);
+  return tiles > 0 ? (tiles + kUnitCost) * a.units : 0;
 }
 
-// Sums over the sequences with all threads: the tiles of all units of all
+// Places of one CTA: an equal share of the line.
+__device__ __forceinline__ int cta_share(int total, int grid) {
+  return static_cast<int>((static_cast<unsigned>(total) + grid - 1) / grid);
+}
+
+// Sums over the sequences with all threads: the places of all
 // sequences, and each thread's exclusive prefix over its own run of `per`
 // sequences. scratch: kAttnWarps values of shared memory.
 template <int TILE>
@@ -171,9 +181,8 @@ __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int* scrat
   mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = threadIdx.x * per + i;
-    if (b < a.B) mine += seq_tiles<TILE>(a, b);
+    if (b < a.B) mine += seq_places<TILE>(a, b);
   }
-  mine *= a.units;
   int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -191,17 +200,20 @@ __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int* scrat
   }
 }
 
-// A place on the line: unit `unit` of sequence b, tile `tile` of its `tiles`.
+// Tile `tile` of unit `unit` of sequence b, and its place on the line.
 template <int TILE>
 struct Cursor {
-  int b, unit, tile, tiles, len, begin;
+  int b, unit, tile, tiles, len, begin, at;
   __device__ __forceinline__ void enter(const AttnArgs& a) {
     len = seq_len(a, b);
     begin = seq_begin(a, len);
     tiles = (len - begin + TILE - 1) / TILE;
   }
+  // The next tile; b == a.B behind the last.
   __device__ __forceinline__ void next(const AttnArgs& a) {
+    ++at;
     if (++tile < tiles) return;
+    at += kUnitCost;
     tile = 0;
     if (++unit < a.units) return;
     unit = 0;
@@ -225,7 +237,7 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int d
 }
 
 template <int DT, int D, bool WIDE>
-__global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool BF16 = DT == D3_DTYPE_BF16;        // type of the matrix products
   constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
@@ -250,21 +262,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   int mine, before, total;
   line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
   const int share = cta_share(total, a.grid);
-  if (blockIdx.x > static_cast<unsigned>((total - 1) / share) || total == 0) return;
-  const int first = blockIdx.x * share;
-  const int count = min(share, total - first);
+  if (total == 0 || static_cast<int64_t>(blockIdx.x) * share >= total) return;
+  const int first = blockIdx.x * share, end = min(first + share, total);
   if (first >= before && first < before + mine) {
     int at = before;
     for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i;
-      const int tiles = seq_tiles<Sh::kTile>(a, b);
-      if (first < at + tiles * a.units) {
+      const int b = tid * per + i, n = seq_places<Sh::kTile>(a, b);
+      if (first < at + n) {
+        const int each = n / a.units, unit = (first - at) / each;
         start[0] = b;
-        start[1] = (first - at) / tiles;
-        start[2] = (first - at) % tiles;
+        start[1] = unit;
+        start[2] = max(0, first - at - unit * each - kUnitCost);
+        start[3] = at + unit * each + kUnitCost + start[2];
         break;
       }
-      at += tiles * a.units;
+      at += n;
     }
   }
   __syncthreads();
@@ -272,6 +284,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   cur.b = start[0];
   cur.unit = start[1];
   cur.tile = start[2];
+  cur.at = start[3];
+  if (cur.at >= end) return;  // nothing but a unit's own places
   cur.enter(a);
   Cursor<Sh::kTile> ld = cur;
 
@@ -306,20 +320,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
       cp_async_16_zfill(dst + ring_at<RB>(r, c), base + (o < 0 ? 0 : o) + c * 16, o >= 0);
     }
   };
-  int loaded = 0;  // tiles whose values have been asked for
   int slot = 0;    // next slot to fill
   auto load_keys = [&]() {
-    if (loaded < count) load(slot, a.k + ld.unit / a.parts * a.k_head, koff);
+    if (ld.at < end) load(slot, a.k + ld.unit / a.parts * a.k_head, koff);
     slot = slot + 1 == S ? 0 : slot + 1;
     cp_async_commit();
   };
   auto load_values = [&]() {
-    if (loaded < count) {
+    if (ld.at < end) {
       load(slot, a.v + ld.unit / a.parts * a.v_head, voff);
-      if (++loaded < count) {
-        ld.next(a);
-        look_up();
-      }
+      ld.next(a);
+      if (ld.at < end) look_up();
     }
     slot = slot + 1 == S ? 0 : slot + 1;
     cp_async_commit();
@@ -360,14 +371,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
   float lg[WIDE ? 2 : 1];  // logit in units of log2 per product
   bool opened = false, whole = false;
   int seg_slot = 0, use = 0;
-  for (int i = 0; i < count; ++i) {
+  bool more = true;
+  for (bool begun = false; more; begun = true) {
     const int head = cur.unit / a.parts;
     const int h0 = head * a.group + (cur.unit % a.parts) * ROWS;
     const int nh = min(ROWS, (head + 1) * a.group - h0);
     if (!opened) {
       opened = true;
       whole = cur.tile == 0;
-      seg_slot = i > 0;
+      seg_slot = begun;
 #pragma unroll
       for (int d = 0; d < DT8; ++d)
 #pragma unroll
@@ -539,15 +551,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
     __syncwarp();  // the same for the values
 
     const bool last = cur.tile + 1 == cur.tiles;
-    if (last || i + 1 == count) {
+    Cursor<Sh::kTile> nxt = cur;
+    nxt.next(a);
+    more = nxt.at < end;
+    if (last || !more) {
       // join the warps: (max, sum) and output rows through shared memory
       opened = false;
-      const bool more = i + 1 < count;
-      Cursor<Sh::kTile> nxt = cur;
-      if (more) {
-        nxt.next(a);
-        fetch_q(nxt);
-      }
+      if (more) fetch_q(nxt);
 #pragma unroll
       for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
         l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
@@ -558,18 +568,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
         }
       }
       __syncthreads();
+      whole = whole && last;
+      float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
+      const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
       // each warp scales its rows to the common maximum; JW at a time they are
       // added into JW buffers, in the order of the warps
-#pragma unroll 1
-      for (int round = 0; round < kAttnWarps / JW; ++round) {
-        if (warp / JW == round) {
 #pragma unroll
-          for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+        if (w) __syncthreads();
+#pragma unroll 1
+        for (int round = 0; round < kAttnWarps / JW; ++round) {
+          if (warp / JW == round) {
             float top = -INFINITY;
 #pragma unroll
             for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, stat[x * 32 + quad + 8 * w]);
             const float f = exp2f(m[w] - (top == -INFINITY ? 0.f : top));
-            float* row = join + ((warp % JW) * ROWS + quad + 8 * w) * JP;
+            float* row = join + ((warp % JW) * 8 + quad) * JP;
             if constexpr (DT == D3_DTYPE_E4M3) {
 #pragma unroll
               for (int d = 0; d < DT8; d += 2) {
@@ -592,47 +606,41 @@ __global__ void __launch_bounds__(kAttnThreads, 1) paged_attention_kernel(const 
               }
             }
           }
+          __syncthreads();
         }
-        __syncthreads();
-      }
-      whole = whole && last;
-      float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
-      const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
-      for (int e = tid * 4; e < ROWS * D; e += kAttnThreads * 4) {
-        const int r = e / D, d = e % D;
-        if (r >= nh) continue;
-        float top = -INFINITY;
+        for (int e = tid * 4; e < 8 * D; e += kAttnThreads * 4) {
+          const int r8 = e / D, d = e % D, r = r8 + 8 * w;
+          if (r >= nh) continue;
+          float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, stat[w * 32 + r]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, x[4] = {};
+          for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, stat[x * 32 + r]);
+          const float base = top == -INFINITY ? 0.f : top;
+          float sum = 0.f, x[4] = {};
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w)
-          sum += exp2f(stat[w * 32 + r] - base) * stat[w * 32 + 16 + r];
+          for (int y = 0; y < kAttnWarps; ++y) sum += exp2f(stat[y * 32 + r] - base) * stat[y * 32 + 16 + r];
 #pragma unroll
-        for (int w = 0; w < JW; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * JP + d);
-          x[0] += y.x;
-          x[1] += y.y;
-          x[2] += y.z;
-          x[3] += y.w;
-        }
-        if (whole) {
-          store_row<QBF16>(a, cur.b, h0 + r, d, x, sum, top, vsc);
-        } else {
-          *reinterpret_cast<float4*>(rec + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-          if (d == 0) {
-            rec[ROWS * D + r] = top;
-            rec[ROWS * D + ROWS + r] = sum;
+          for (int z = 0; z < JW; ++z) {
+            const float4 y = *reinterpret_cast<const float4*>(join + (z * 8 + r8) * JP + d);
+            x[0] += y.x;
+            x[1] += y.y;
+            x[2] += y.z;
+            x[3] += y.w;
+          }
+          if (whole) {
+            store_row<QBF16>(a, cur.b, h0 + r, d, x, sum, top, vsc);
+          } else {
+            *reinterpret_cast<float4*>(rec + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d == 0) {
+              rec[ROWS * D + r] = top;
+              rec[ROWS * D + ROWS + r] = sum;
+            }
           }
         }
       }
       if (more) place_q();  // every warp took its queries before the barriers above
-      cur = nxt;
       __syncthreads();
-    } else {
-      ++cur.tile;
     }
+    cur = nxt;
   }
   cp_async_wait<0>();
 }
@@ -663,19 +671,19 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   const int tiles = seq_tiles<Sh::kTile>(a, b);
   if (b / per == tid) {
     int at = before;
-    for (int x = tid * per; x < b; ++x) at += seq_tiles<Sh::kTile>(a, x) * a.units;
-    *found = at + unit * tiles;
+    for (int x = tid * per; x < b; ++x) at += seq_places<Sh::kTile>(a, x);
+    *found = at + unit * (tiles + kUnitCost);
   }
   __syncthreads();
-  const int share = cta_share(total, a.grid);
-  const int lo = *found, hi = lo + tiles;  // the unit's tiles on the line
-  const int c0 = lo / share, n = tiles > 0 ? (hi - 1) / share - c0 + 1 : 0;
+  const int share = max(1, cta_share(total, a.grid));
+  const int lo = *found, hi = lo + kUnitCost + tiles;  // the unit's places on the line
+  const int c0 = (lo + kUnitCost) / share, n = tiles > 0 ? (hi - 1) / share - c0 + 1 : 0;
   // every CTA waits: a kernel after this one waits for this grid only, which
   // must not be complete before the main kernel is
   pdl_wait();
   if (n == 1) return;
   // the first record lies in its CTA's second place where the CTA began with another unit
-  const float* rec0 = a.partial + (static_cast<int64_t>(c0) * 2 + (lo != c0 * share)) * Sh::kRecord;
+  const float* rec0 = a.partial + (static_cast<int64_t>(c0) * 2 + (lo > c0 * share)) * Sh::kRecord;
   const float* rec = a.partial + static_cast<int64_t>(c0) * 2 * Sh::kRecord;  // + 2 c records, c > 0
   auto record = [&](int c) { return c == 0 ? rec0 : rec + static_cast<int64_t>(c) * 2 * Sh::kRecord; };
   float top = -INFINITY, sum = 0.f;
@@ -762,7 +770,7 @@ extern "C" int d3_paged_attention_workspace_size(int B, int q_heads, int kv_head
              "query heads must be a multiple of key heads");
   D3_REQUIRE(dim == 64 || dim == 128 || dim == 256, "head dim must be 64, 128 or 256");
   const int rows = q_heads / kv_heads > 8 ? 16 : 8;
-  *bytes = static_cast<size_t>(sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
+  *bytes = static_cast<size_t>(2 * sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
   return D3_OK;
 }
 
@@ -820,12 +828,12 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   a.units = cache->heads * a.parts;
   a.scale = scale;
   a.partial = static_cast<float*>(workspace);
-  a.grid = sm_count();
+  a.grid = 2 * sm_count();
   a.status = status;
   D3_REQUIRE(aligned(q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0, "rows of q must be 16-byte aligned");
   D3_REQUIRE(aligned(out, 8) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0, "rows of out must be 8-byte aligned");
   // the line of tiles (64 keys at least, see AttnShape) is counted in 32 bits
-  D3_REQUIRE(static_cast<int64_t>(B) * a.units * (a.max_len / 64 + 1) < 0x40000000 &&
+  D3_REQUIRE(static_cast<int64_t>(B) * a.units * (a.max_len / 64 + 2) < 0x40000000 &&
                  static_cast<int64_t>(B) * q_heads <= 0x7fffffff,
              "batch, heads and length are too large for one call");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
