@@ -1,0 +1,78 @@
+// Shared-memory tiles and mma.sync m16n8k16 fragments of the 16-bit kernels that
+// keep their accumulators in registers (attention and the gated delta rule).
+#pragma once
+
+#include "d3_common.cuh"
+
+namespace d3 {
+
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1,
+                                                  uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+// c += A(16x16, row) * B(16x8, col) for bf16 or f16 operands.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  } else {
+    const __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float unpack16(uint16_t b) {
+  if constexpr (BF16) return bf16_bits_to_f32(b);
+  return __half2float(__ushort_as_half(b));
+}
+
+// Byte offset of 16-byte piece c of row r of a shared-memory tile: pieces are permuted so
+// that the 8 rows of an ldmatrix tile fall into different banks.
+template <int ROW_BYTES>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  constexpr int kPieces = ROW_BYTES / 16;
+  const int x = kPieces >= 8 ? (r & 7) : ((r >> 1) & 3);  // 64-byte rows share a 128-byte line
+  return r * ROW_BYTES + ((c ^ x) << 4);
+}
+
+// v = hi + lo to 2^-17: two values as a pair of bf16x2 words.
+__device__ __forceinline__ void split_bf16x2(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack16<true>(v0, v1);
+  lo = pack16<true>(v0 - __uint_as_float(hi << 16), v1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+// Four 8x8 b16 tiles written transposed: row r of a tile in memory is its column r.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0),
+               "r"(r1), "r"(r2), "r"(r3)
+               : "memory");
+}
+
+}  // namespace d3

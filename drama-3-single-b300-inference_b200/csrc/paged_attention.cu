@@ -28,6 +28,7 @@
 // a power of two per row into f16's range (exact for every element within 2^-14
 // of the row's largest, error below 2^-25 of that otherwise).
 #include "kv_cache.cuh"
+#include "mma_tiles.cuh"
 
 namespace d3 {
 namespace {
@@ -87,62 +88,6 @@ struct AttnShape {
   static_assert(kSmem <= kMaxSmem);
   static constexpr int kRecord = kRows * (D + 2);  // floats of a partial result
 };
-
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1,
-                                                  uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-
-// c += A(16x16, row) * B(16x8, col) for bf16 or f16 operands.
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-  } else {
-    const __half2 p = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ float unpack16(uint16_t b) {
-  if constexpr (BF16) return bf16_bits_to_f32(b);
-  return __half2float(__ushort_as_half(b));
-}
-
-// Byte offset of 16-byte piece c of row r in a stage: pieces are permuted so
-// that the 8 rows of an ldmatrix tile fall into different banks.
-template <int ROW_BYTES>
-__device__ __forceinline__ uint32_t ring_at(int r, int c) {
-  constexpr int kPieces = ROW_BYTES / 16;
-  const int x = kPieces >= 8 ? (r & 7) : ((r >> 1) & 3);  // 64-byte rows share a 128-byte line
-  return r * ROW_BYTES + ((c ^ x) << 4);
-}
 
 __device__ __forceinline__ int seq_begin(const AttnArgs& a, int len) {
   return a.window > 0 ? max(0, len - a.window) : 0;
@@ -317,7 +262,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
     for (int it = 0; it < NK * PIECES / 32; ++it) {
       const int idx = it * 32 + lane, r = idx / PIECES, c = idx % PIECES;
       const int64_t o = __shfl_sync(0xffffffffu, mine_off, r);
-      cp_async_16_zfill(dst + ring_at<RB>(r, c), base + (o < 0 ? 0 : o) + c * 16, o >= 0);
+      cp_async_16_zfill(dst + tile_at<RB>(r, c), base + (o < 0 ? 0 : o) + c * 16, o >= 0);
     }
   };
   int slot = 0;    // next slot to fill
@@ -441,7 +386,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
           uint32_t b[4];
-          ldmatrix_x4(ks + ring_at<RB>(n * 8 + mtop * 8 + mrow, c + mhi), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4(ks + tile_at<RB>(n * 8 + mtop * 8 + mrow, c + mhi), b[0], b[1], b[2], b[3]);
 #pragma unroll
           for (int y = 0; y < 2; ++y)    // k step
 #pragma unroll
@@ -458,7 +403,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
           uint32_t b[4];
-          ldmatrix_x4(ks + ring_at<RB>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4(ks + tile_at<RB>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if constexpr (WIDE) mma_16816<BF16>(s[n + x], qf[c][0], qf[c][1], qf[c][2], qf[c][3], b[2 * x], b[2 * x + 1]);
@@ -523,7 +468,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
 #pragma unroll
         for (int c = 0; c < D / 16; c += 2) {
           uint32_t b[4];
-          ldmatrix_x4_trans(vs + ring_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4_trans(vs + tile_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             // a 16-bit unit holds two neighbouring columns of a key: even and
@@ -543,7 +488,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
 #pragma unroll
         for (int c = 0; c < DT8; c += 2) {
           uint32_t b[4];
-          ldmatrix_x4_trans(vs + ring_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4_trans(vs + tile_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
           mma_16816<BF16>(o[c], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[0], b[1]);
           mma_16816<BF16>(o[c + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[2], b[3]);
         }
