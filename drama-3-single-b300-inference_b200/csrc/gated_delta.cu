@@ -17,9 +17,12 @@
 // and then
 //   out_i = exp(G_i) S0^T q_i + sum_{j<=i} P_ij n_j,   P_ij = exp(G_i - G_j) q_i.k_j,
 //   S1 = exp(G_64) S0 + sum_j exp(G_64 - G_j) k_j n_j^T.
-// A first kernel makes T = (I + A)^-1 diag(beta) and P for all chunks in parallel
-// (they do not need the state); a second one walks each sequence's chunks with the
-// state in registers. What follows from products of 16-bit factors runs on
+// The first equation is solved in two halves of 32 tokens: with T_h the inverse of
+// I + A's diagonal block h, times diag(beta), and B_ij = exp(G_i - G_j) k_i.k_j,
+//   N_0 = T_0 R_0,   N_1 = T_1 (R_1 - B_10 N_0).
+// A first kernel makes T_0, T_1, B_10 and P for all chunks in parallel (they do not
+// need the state); a second one walks each sequence's chunks with the state in
+// registers. What follows from products of 16-bit factors runs on
 // mma.sync; the state has to stay exact to fp32's neighbourhood, so every factor of
 // a product that reaches it (S0, R, N, T) is split into two bf16 terms (2^-17),
 // and the keys are taken as they come, bf16, with their norms as factors outside.
@@ -48,6 +51,13 @@ struct DeltaArgs {
   float scale, eps;
   int32_t* status;
 };
+
+// 2^x, results below 2^-126 as zero (decays: they are added to what they vanish beside).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // State slot of sequence i, or -1 when it is left out.
 __device__ __forceinline__ int delta_slot(const DeltaArgs& a, int i) {
@@ -159,10 +169,11 @@ __global__ void __launch_bounds__(kDeltaThreads)
 
 // ------------------------------------------------------------------ chunks --
 constexpr int kC = 64;              // tokens of a chunk
-constexpr int kPrepThreads = 128;
-// What the first kernel leaves for one (chunk, value head): T in two bf16 terms
-// and P, row-major 64 x 64 (16 x 16 blocks above the diagonal are not written), then the
-// tokens' factors exp(G) / |k|, exp(G) scale / |q|, exp(G_64 - G) / |k| and exp(G_64).
+constexpr int kPrepThreads = 256;
+// What the first kernel leaves for one (chunk, value head): the matrix [T_0 0; B_10 T_1]
+// in two bf16 terms and P in one, row-major 64 x 64 (16 x 16 blocks above the diagonal
+// are not written), then the tokens' factors exp(G) / |k|, exp(G) scale / |q|,
+// exp(G_64 - G) / |k| and exp(G_64).
 constexpr int kRecT = kC * kC * 2, kRecScal = 3 * kRecT, kRecBytes = kRecScal + 1024;
 
 // The chunks of sequence i have records cu[i] / 64 + i, ...: no two sequences share
@@ -190,27 +201,29 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const __nv_bfloat16* sr
   }
 }
 
-constexpr int kLd = 68;  // floats between rows of the 64 x 64 fp32 matrices
+constexpr int kLd = 36;  // floats between rows of the fp32 matrices: 64 rows of a 32 x 32 block each
 
 template <int DK>
 struct PrepShape {
   static constexpr int kTile = kC * DK * 2;
-  static constexpr int kT = kC * kLd * 4 + 32 * 36 * 4;  // T and a 32 x 32 product, over the dead tiles
+  static constexpr int kMat = kC * kLd * 4;
+  static constexpr int kT = 2 * kMat + 2 * 32 * 20 * 4;  // two heads' T and 16 x 16 products, over the dead tiles
   static constexpr int kTiles = 2 * kTile > kT ? 2 * kTile : kT;
-  static constexpr int kSmem = kTiles + kC * kLd * 4 + 6 * kC * 4;
+  static constexpr int kSmem = kTiles + 2 * kMat + (2 * kC * 2 + 2 * kC + 8) * 4;
 };
 
-// One CTA per (record, key head): T, P and the factors of its value heads.
+// One CTA per (record, key head), two of its value heads at a time. Warps 0-3 make
+// k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads share them.
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads) gated_delta_prep_kernel(const ChunkArgs a) {
+__global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const ChunkArgs a) {
   using Sh = PrepShape<DK>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* Tm = reinterpret_cast<float*>(smem);
-  float* X = Tm + kC * kLd;
-  float* A = reinterpret_cast<float*>(smem + Sh::kTiles);
-  float* sG = A + kC * kLd;  // sums of g, in units of log2
-  float* sB = sG + kC;
-  float* sRk = sB + kC;
+  float* Tm = reinterpret_cast<float*>(smem);                    // [2][64][kLd]
+  float* X = Tm + 2 * kC * kLd;                                  // [2][32][20]
+  float* A = reinterpret_cast<float*>(smem + Sh::kTiles);        // [2][64][kLd]
+  float* sG = A + 2 * kC * kLd;  // [2][64] sums of g, in units of log2
+  float* sB = sG + 2 * kC;       // [2][64]
+  float* sRk = sB + 2 * kC;
   float* sRq = sRk + kC;
   float* sScan = sRq + kC;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
@@ -234,238 +247,266 @@ __global__ void __launch_bounds__(kPrepThreads) gated_delta_prep_kernel(const Ch
   load_rows<DK * 2, kPrepThreads>(kt, d.k + hk * DK, d.k_stride, t0, c1);
   load_rows<DK * 2, kPrepThreads>(qt, d.q + hk * DK, d.q_stride, t0, c1);
   cp_async_commit();
+  // decays and step sizes of the first two heads, on their way meanwhile
+  const int gh = tid >> 6, gt = tid & (kC - 1);  // (threads 0-127) head, token
+  auto fetch = [&](const float* x, int64_t stride, int hv) {
+    return gt < nt && hv < (hk + 1) * d.rep ? __ldg(x + (t0 + gt) * stride + hv) : 0.f;
+  };
+  float g_next = 0.f, b_next = 0.f;
+  if (tid < 2 * kC) {
+    g_next = fetch(d.g, d.g_stride, hk * d.rep + gh);
+    b_next = fetch(d.beta, d.beta_stride, hk * d.rep + gh);
+  }
   cp_async_wait<0>();
   __syncthreads();
-  // norms: two threads per row
+  const int role = warp >> 2, rows = 16 * (warp & 3);
+  // norms: two threads per row of k (warps 0-3) or q
   {
-    const int r = tid >> 1;
-    float kk = 0.f, qq = 0.f;
+    const int r = (tid & 127) >> 1;
+    float xx = 0.f;
 #pragma unroll
     for (int c = 0; c < DK / 16; ++c) {
-      const uint32_t at = tile_at<DK * 2>(r, c * 2 + (tid & 1));
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + at), y = *reinterpret_cast<const uint4*>(smem + Sh::kTile + at);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + role * Sh::kTile + tile_at<DK * 2>(r, c * 2 + (tid & 1)));
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        kk = fma_bf16x2_seq(xs[i], xs[i], kk);
-        qq = fma_bf16x2_seq(ys[i], ys[i], qq);
-      }
+      for (int i = 0; i < 4; ++i) xx = fma_bf16x2_seq(xs[i], xs[i], xx);
     }
-    kk += __shfl_xor_sync(0xffffffffu, kk, 1);
-    qq += __shfl_xor_sync(0xffffffffu, qq, 1);
-    if ((tid & 1) == 0) {
-      const bool in = r < nt;
-      sRk[r] = !in ? 0.f : d.l2norm ? rsqrtf(kk + d.eps) : 1.f;
-      sRq[r] = !in ? 0.f : d.scale * (d.l2norm ? rsqrtf(qq + d.eps) : 1.f);
-    }
+    xx += __shfl_xor_sync(0xffffffffu, xx, 1);
+    const float f = d.l2norm ? rsqrtf(xx + d.eps) : 1.f;
+    if ((tid & 1) == 0) (role ? sRq : sRk)[r] = r < nt ? (role ? d.scale * f : f) : 0.f;
   }
-  // k_i.k_j and q_i.k_j of rows 16 warp .. + 15, columns up to the diagonal block
-  float kk[8][4], qk[8][4];
+  // products of rows `rows` .. + 15 with the keys up to the diagonal block
+  float acc[8][4];
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) kk[n][x] = qk[n][x] = 0.f;
+    for (int x = 0; x < 4; ++x) acc[n][x] = 0.f;
   const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
 #pragma unroll
   for (int c = 0; c < DK / 16; ++c) {
-    uint32_t ak[4], aq[4];
+    uint32_t x[4];
     // A operand: tiles (rows 0-7, k 0-7), (rows 8-15, k 0-7), (rows 0-7, k 8-15), (rows 8-15, k 8-15)
-    const uint32_t at = tile_at<DK * 2>(16 * warp + mhi * 8 + mrow, 2 * c + mtop);
-    ldmatrix_x4(kt + at, ak[0], ak[1], ak[2], ak[3]);
-    ldmatrix_x4(qt + at, aq[0], aq[1], aq[2], aq[3]);
+    ldmatrix_x4(kt + role * Sh::kTile + tile_at<DK * 2>(rows + mhi * 8 + mrow, 2 * c + mtop), x[0], x[1], x[2], x[3]);
 #pragma unroll
     for (int n = 0; n < 8; n += 2) {
-      if (n > 2 * warp) break;
+      if (n * 8 > rows) break;
       uint32_t b[4];
       ldmatrix_x4(kt + tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        mma_16816<true>(kk[n + x], ak[0], ak[1], ak[2], ak[3], b[2 * x], b[2 * x + 1]);
-        mma_16816<true>(qk[n + x], aq[0], aq[1], aq[2], aq[3], b[2 * x], b[2 * x + 1]);
-      }
+      mma_16816<true>(acc[n], x[0], x[1], x[2], x[3], b[0], b[1]);
+      mma_16816<true>(acc[n + 1], x[0], x[1], x[2], x[3], b[2], b[3]);
     }
   }
-  for (int hv = hk * d.rep; hv < (hk + 1) * d.rep; ++hv) {
-    uint8_t* rec = a.rec + (static_cast<int64_t>(blockIdx.x) * d.value_heads + hv) * kRecBytes;
-    __syncthreads();  // the tiles, or the previous head's matrices, are no longer read
+  for (int hv0 = hk * d.rep; hv0 < (hk + 1) * d.rep; hv0 += 2) {
+    const int heads = min(2, (hk + 1) * d.rep - hv0);
+    uint8_t* rec0 = a.rec + (static_cast<int64_t>(blockIdx.x) * d.value_heads + hv0) * kRecBytes;
+    __syncthreads();  // the tiles, or the previous heads' matrices, are no longer read
     float G = 0.f;
-    if (tid < kC) {
-      G = tid < nt ? __ldg(d.g + (t0 + tid) * d.g_stride + hv) * 1.4426950408889634f : 0.f;
-      sB[tid] = tid < nt ? __ldg(d.beta + (t0 + tid) * d.beta_stride + hv) : 0.f;
+    if (tid < 2 * kC) {
+      G = g_next * 1.4426950408889634f;
+      sB[tid] = b_next;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const float y = __shfl_up_sync(0xffffffffu, G, o);
         if (lane >= o) G += y;
       }
       if (lane == 31) sScan[warp] = G;
+      g_next = fetch(d.g, d.g_stride, hv0 + 2 + gh);
+      b_next = fetch(d.beta, d.beta_stride, hv0 + 2 + gh);
     }
     __syncthreads();
-    if (tid < kC) {
-      if (warp == 1) G += sScan[0];
+    if (tid < 2 * kC) {
+      if (warp & 1) G += sScan[warp - 1];
       sG[tid] = G;
     }
     __syncthreads();
-    if (tid < kC) {
-      float* f = reinterpret_cast<float*>(rec + kRecScal);
-      const float end = sG[kC - 1];
-      f[tid] = exp2f(G) * sRk[tid];
-      f[kC + tid] = exp2f(G) * sRq[tid];
-      f[2 * kC + tid] = exp2f(end - G) * sRk[tid];
-      if (tid == 0) f[3 * kC] = exp2f(end);
+    if (tid < 2 * kC && gh < heads) {
+      float* f = reinterpret_cast<float*>(rec0 + gh * kRecBytes + kRecScal);
+      const float end = sG[gh * kC + kC - 1];
+      f[gt] = exp2_fast(G) * sRk[gt];
+      f[kC + gt] = exp2_fast(G) * sRq[gt];
+      f[2 * kC + gt] = exp2_fast(end - G) * sRk[gt];
+      if (gt == 0) f[3 * kC] = exp2_fast(end);
     }
+    for (int h = 0; h < heads; ++h) {
+      uint8_t* rec = rec0 + h * kRecBytes;
+      const float *hG = sG + h * kC, *hB = sB + h * kC;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int i = 16 * warp + quad + 8 * half;
-      const float gi = sG[i], bi = sB[i] * sRk[i], qi = sRq[i];
+      for (int half = 0; half < 2; ++half) {
+        const int i = rows + quad + 8 * half;
+        const float gi = hG[i], fi = role ? sRq[i] : sRk[i], bi = hB[i];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (n > 2 * warp + 1) break;
-        const int j = n * 8 + 2 * t4;
-        float p[2], w[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float e = j + x <= i ? exp2f(gi - sG[j + x]) * sRk[j + x] : 0.f;
-          w[x] = j + x < i ? bi * e * kk[n][2 * half + x] : 0.f;
-          p[x] = j + x <= i ? qi * e * qk[n][2 * half + x] : 0.f;
+        for (int n = 0; n < 8; ++n) {
+          if (n * 8 > rows + 8) break;
+          const int j = n * 8 + 2 * t4;
+          const float2 gj = *reinterpret_cast<const float2*>(hG + j), rj = *reinterpret_cast<const float2*>(sRk + j);
+          // exp(G_i - G_j) times the two norms
+          float e0 = exp2_fast(gi - gj.x) * (rj.x * fi) * acc[n][2 * half];
+          float e1 = exp2_fast(gi - gj.y) * (rj.y * fi) * acc[n][2 * half + 1];
+          if (n * 8 >= rows) {  // the diagonal block: nothing above (there the difference may overflow)
+            e0 = j <= i ? e0 : 0.f;
+            e1 = j + 1 <= i ? e1 : 0.f;
+          }
+          if (role) {
+            *reinterpret_cast<uint32_t*>(rec + 2 * kRecT + (i * kC + j) * 2) = pack16<true>(e0, e1);
+          } else if (rows >= 32 && n < 4) {
+            uint32_t x, y;
+            split_bf16x2(e0, e1, x, y);
+            *reinterpret_cast<uint32_t*>(rec + (i * kC + j) * 2) = x;
+            *reinterpret_cast<uint32_t*>(rec + kRecT + (i * kC + j) * 2) = y;
+          } else {
+            *reinterpret_cast<float2*>(A + (h * kC + i) * kLd + (j & 31)) = make_float2(j < i ? e0 * bi : 0.f, j + 1 < i ? e1 * bi : 0.f);
+          }
         }
-        *reinterpret_cast<float2*>(A + i * kLd + j) = make_float2(w[0], w[1]);
-        *reinterpret_cast<uint32_t*>(rec + 2 * kRecT + (i * kC + j) * 2) = pack16<true>(p[0], p[1]);
       }
     }
     __syncthreads();
-    // T = (I + A)^-1. Diagonal blocks of 16: thread (block, column) substitutes forward.
-    if (tid < kC) {
-      const int b = tid >> 4, c = tid & 15;
-      const float* Ab = A + (16 * b) * kLd + 16 * b;
-      float x[16];
+    // (I + A)^-1 of the diagonal blocks of 16, one per warp: columns of the two blocks of
+    // 8 by forward substitution, then [T1 0; -T2 A21 T1, T2]
+    if ((warp >> 2) < heads) {
+      const int b = warp & 3, at = ((warp >> 2) * kC + 16 * b) * kLd + 16 * (b & 1);
+      const float* Ab = A + at;
+      float *Tb = Tm + at, *Xb = X + warp * 160;
+      if (lane < 16) {
+        const int o = lane & 8, c = lane & 7;
+        float x[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float s = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          float y = 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) s = fmaf(Ab[i * kLd + j], x[j], s);
-        x[i] = i < c ? 0.f : i == c ? 1.f : -s;
-        Tm[(16 * b + i) * kLd + 16 * b + c] = x[i];
+          for (int j = 0; j < i; ++j) y = fmaf(Ab[(o + i) * kLd + o + j], x[j], y);
+          x[i] = i < c ? 0.f : i == c ? 1.f : -y;
+          Tb[(o + i) * kLd + o + c] = x[i];
+        }
       }
+      __syncwarp();
+      const int r = lane >> 2, c = (lane & 3) * 2;
+      float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = Ab[(8 + r) * kLd + k];
+        const float2 y = *reinterpret_cast<const float2*>(Tb + k * kLd + c);
+        x0 = fmaf(w, y.x, x0);
+        x1 = fmaf(w, y.y, x1);
+      }
+      *reinterpret_cast<float2*>(Xb + r * 20 + c) = make_float2(x0, x1);
+      __syncwarp();
+      x0 = x1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = Tb[(8 + r) * kLd + 8 + k];
+        const float2 y = *reinterpret_cast<const float2*>(Xb + k * 20 + c);
+        x0 = fmaf(w, y.x, x0);
+        x1 = fmaf(w, y.y, x1);
+      }
+      *reinterpret_cast<float2*>(Tb + (8 + r) * kLd + c) = make_float2(-x0, -x1);
+      *reinterpret_cast<float2*>(Tb + r * kLd + 8 + c) = make_float2(0.f, 0.f);  // read by the next level
     }
     __syncthreads();
-    // [T1 0; -T2 A21 T1, T2] from 16 to 32
+    // from 16 to 32: [T1 0; -T2 A21 T1, T2]
     {
-      const int p = tid >> 6, r = (tid & 63) >> 2, c = (tid & 3) * 4, o = 32 * p;
+      const int h = tid >> 7, p = (tid >> 6) & 1, r = (tid & 63) >> 2, c = (tid & 3) * 4;
+      const float* Ah = A + (h * kC + 32 * p) * kLd;
+      float* Th = Tm + (h * kC + 32 * p) * kLd;
+      float* Xh = X + (h * 32 + 16 * p) * 20;
       float x[4] = {};
+      if (h < heads) {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float w = A[(o + 16 + r) * kLd + o + k];
-        const float4 y = *reinterpret_cast<const float4*>(Tm + (o + k) * kLd + o + c);
-        x[0] = fmaf(w, y.x, x[0]); x[1] = fmaf(w, y.y, x[1]); x[2] = fmaf(w, y.z, x[2]); x[3] = fmaf(w, y.w, x[3]);
+        for (int k = 0; k < 16; ++k) {
+          const float w = Ah[(16 + r) * kLd + k];
+          const float4 y = *reinterpret_cast<const float4*>(Th + k * kLd + c);
+          x[0] = fmaf(w, y.x, x[0]); x[1] = fmaf(w, y.y, x[1]); x[2] = fmaf(w, y.z, x[2]); x[3] = fmaf(w, y.w, x[3]);
+        }
+        *reinterpret_cast<float4*>(Xh + r * 20 + c) = make_float4(x[0], x[1], x[2], x[3]);
       }
-      *reinterpret_cast<float4*>(X + (16 * p + r) * 36 + c) = make_float4(x[0], x[1], x[2], x[3]);
       __syncthreads();
-      float y[4] = {};
+      if (h < heads) {
+        float y[4] = {};
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float w = Tm[(o + 16 + r) * kLd + o + 16 + k];
-        const float4 z = *reinterpret_cast<const float4*>(X + (16 * p + k) * 36 + c);
-        y[0] = fmaf(w, z.x, y[0]); y[1] = fmaf(w, z.y, y[1]); y[2] = fmaf(w, z.z, y[2]); y[3] = fmaf(w, z.w, y[3]);
+        for (int k = 0; k < 16; ++k) {
+          const float w = Th[(16 + r) * kLd + 16 + k];
+          const float4 z = *reinterpret_cast<const float4*>(Xh + k * 20 + c);
+          y[0] = fmaf(w, z.x, y[0]); y[1] = fmaf(w, z.y, y[1]); y[2] = fmaf(w, z.z, y[2]); y[3] = fmaf(w, z.w, y[3]);
+        }
+        *reinterpret_cast<float4*>(Th + (16 + r) * kLd + c) = make_float4(-y[0], -y[1], -y[2], -y[3]);
       }
-      *reinterpret_cast<float4*>(Tm + (o + 16 + r) * kLd + o + c) = make_float4(-y[0], -y[1], -y[2], -y[3]);
-      // the block above the diagonal is read by the next level
-      *reinterpret_cast<float4*>(Tm + (o + r) * kLd + o + 16 + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __syncthreads();
-    // and from 32 to 64
-    {
-      const int r = tid >> 2, c = (tid & 3) * 8;
-      float x[8] = {};
-#pragma unroll 8
-      for (int k = 0; k < 32; ++k) {
-        const float w = A[(32 + r) * kLd + k];
-        const float4 y = *reinterpret_cast<const float4*>(Tm + k * kLd + c), z = *reinterpret_cast<const float4*>(Tm + k * kLd + c + 4);
-        x[0] = fmaf(w, y.x, x[0]); x[1] = fmaf(w, y.y, x[1]); x[2] = fmaf(w, y.z, x[2]); x[3] = fmaf(w, y.w, x[3]);
-        x[4] = fmaf(w, z.x, x[4]); x[5] = fmaf(w, z.y, x[5]); x[6] = fmaf(w, z.z, x[6]); x[7] = fmaf(w, z.w, x[7]);
-      }
-      *reinterpret_cast<float4*>(X + r * 36 + c) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4*>(X + r * 36 + c + 4) = make_float4(x[4], x[5], x[6], x[7]);
-      __syncthreads();
-      float u[8] = {};
-#pragma unroll 8
-      for (int k = 0; k < 32; ++k) {
-        const float w = Tm[(32 + r) * kLd + 32 + k];
-        const float4 y = *reinterpret_cast<const float4*>(X + k * 36 + c), z = *reinterpret_cast<const float4*>(X + k * 36 + c + 4);
-        u[0] = fmaf(w, y.x, u[0]); u[1] = fmaf(w, y.y, u[1]); u[2] = fmaf(w, y.z, u[2]); u[3] = fmaf(w, y.w, u[3]);
-        u[4] = fmaf(w, z.x, u[4]); u[5] = fmaf(w, z.y, u[5]); u[6] = fmaf(w, z.z, u[6]); u[7] = fmaf(w, z.w, u[7]);
-      }
-      *reinterpret_cast<float4*>(Tm + (32 + r) * kLd + c) = make_float4(-u[0], -u[1], -u[2], -u[3]);
-      *reinterpret_cast<float4*>(Tm + (32 + r) * kLd + c + 4) = make_float4(-u[4], -u[5], -u[6], -u[7]);
     }
     __syncthreads();
     // T diag(beta) in two bf16 terms, 8 elements at a time
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = (e * kPrepThreads + tid) >> 3, j = (tid & 7) * 8;
-      if (j >= (i & ~15) + 16) continue;
-      uint32_t h[4], l[4];
+    for (int e = 0; e < 2; ++e) {
+      const int x = e * kPrepThreads + tid, h = x >> 8, i = (x >> 2) & (kC - 1), j = (x & 3) * 8;
+      if (h >= heads || j >= (i & 16) + 16) continue;
+      const float *row = Tm + (h * kC + i) * kLd + j, *hB = sB + h * kC + (i & 32) + j;
+      uint32_t p[4], q[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        split_bf16x2(Tm[i * kLd + j + 2 * x] * sB[j + 2 * x], Tm[i * kLd + j + 2 * x + 1] * sB[j + 2 * x + 1], h[x], l[x]);
-      *reinterpret_cast<uint4*>(rec + (i * kC + j) * 2) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(rec + kRecT + (i * kC + j) * 2) = make_uint4(l[0], l[1], l[2], l[3]);
+      for (int y = 0; y < 4; ++y) split_bf16x2(row[2 * y] * hB[2 * y], row[2 * y + 1] * hB[2 * y + 1], p[y], q[y]);
+      uint8_t* at = rec0 + h * kRecBytes + (i * kC + (i & 32) + j) * 2;
+      *reinterpret_cast<uint4*>(at) = make_uint4(p[0], p[1], p[2], p[3]);
+      *reinterpret_cast<uint4*>(at + kRecT) = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
 }
 
-template <int DK, int WARPS>
+constexpr int kWalkWarps = 4, kWalkThreads = kWalkWarps * 32, kWalkCols = 16 * kWalkWarps;
+
+// Two CTAs share an SM: keys, queries, values and factors of two chunks, and T and P of
+// one, whose place is free again by the time the state is updated.
+template <int DK>
 struct WalkShape {
-  static constexpr int kKT = kC * DK * 2, kVRow = WARPS * 32;
-  static constexpr int kV = kC * kVRow;
-  static constexpr int kK = 0, kQ = kKT, kRec = 2 * kKT, kVAt = kRec + kRecBytes, kStage = kVAt + kV;
-  static constexpr int kOut = 2 * kStage;                 // 2 KB per warp
-  static constexpr int kSmem = kOut + WARPS * 2048;
+  static constexpr int kKT = kC * DK * 2, kV = kC * kWalkCols * 2;
+  static constexpr int kQ = kKT, kVAt = 2 * kKT, kF = kVAt + kV, kStage = kF + 1024;
+  static constexpr int kRec = 2 * kStage;
+  static constexpr int kSmem = kRec + 3 * kRecT;
+  static_assert(kSmem <= 113 * 1024);
 };
 
-// One CTA per (16 WARPS value columns, value head, sequence) walks the sequence's
+// One CTA per (64 value columns, value head, sequence) walks the sequence's
 // chunks. Warp w holds the transposed state of its 16 value columns, [16, DK], as
 // mma accumulators: these are laid out like A operands, so the state, R and N go from
 // product to product in registers, and warps share only what they read (keys,
 // queries, T, P), which cp.async brings one chunk ahead.
-template <int DK, int DV, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const ChunkArgs a) {
-  using Sh = WalkShape<DK, WARPS>;
-  constexpr int THREADS = WARPS * 32, VR = Sh::kVRow;
+template <int DK, int DV>
+__global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const ChunkArgs a) {
+  using Sh = WalkShape<DK>;
+  constexpr int VR = kWalkCols * 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
   const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
   const DeltaArgs& d = a.d;
   const int seq = blockIdx.z, hv = blockIdx.y, hk = hv / d.rep;
-  const int col = blockIdx.x * WARPS * 16;  // first value column of the CTA
+  const int col = blockIdx.x * kWalkCols;  // first value column of the CTA
   pdl_wait();
   pdl_trigger();
   const int c0 = max(0, __ldg(a.cu + seq)), c1 = min(a.T, __ldg(a.cu + seq + 1));
   const int slot = delta_slot(d, seq);
   if (slot < 0) {
-    for (int e = tid; e < (c1 - c0) * WARPS * 2; e += THREADS)
-      *reinterpret_cast<uint4*>(d.out + (c0 + e / (WARPS * 2)) * d.out_stride + hv * DV + col + e % (WARPS * 2) * 8) = make_uint4(0, 0, 0, 0);
+    for (int e = tid; e < (c1 - c0) * (kWalkCols / 8); e += kWalkThreads)
+      *reinterpret_cast<uint4*>(d.out + (c0 + e / (kWalkCols / 8)) * d.out_stride + hv * DV + col + e % (kWalkCols / 8) * 8) = make_uint4(0, 0, 0, 0);
     return;
   }
   const uint8_t* rec = a.rec + (first_record(c0, seq) * d.value_heads + hv) * kRecBytes;
   const int64_t rec_step = static_cast<int64_t>(d.value_heads) * kRecBytes;
-  auto load = [&](int stage, int t0) {
-    const uint32_t s = smem_u32(smem) + stage * Sh::kStage;
-    load_rows<DK * 2, THREADS>(s + Sh::kK, d.k + hk * DK, d.k_stride, t0, c1);
-    load_rows<DK * 2, THREADS>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1);
-    load_rows<VR, THREADS>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1);
-    // T (two terms) and P: blocks up to the diagonal
+  const uint32_t sm = smem_u32(smem);
+  auto load_tokens = [&](int stage, int t0, const uint8_t* rec) {
+    const uint32_t s = sm + stage * Sh::kStage;
+    load_rows<DK * 2, kWalkThreads>(s, d.k + hk * DK, d.k_stride, t0, c1);
+    load_rows<DK * 2, kWalkThreads>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1);
+    load_rows<VR, kWalkThreads>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1);
+    if (tid < 49) cp_async_16(smem + stage * Sh::kStage + Sh::kF + tid * 16, rec + kRecScal + tid * 16);
+  };
+  auto load_matrices = [&](const uint8_t* rec) {  // blocks up to the diagonal
 #pragma unroll
-    for (int i = 0; i < 3 * kC * 8 / THREADS; ++i) {
-      const int e = i * THREADS + tid, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
-      if (c < (r >> 4) * 2 + 2) cp_async_16(smem + stage * Sh::kStage + Sh::kRec + m * kRecT + tile_at<128>(r, c), rec + m * kRecT + r * 128 + c * 16);
+    for (int i = 0; i < 3 * kC * 8 / kWalkThreads; ++i) {
+      const int e = i * kWalkThreads + tid, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
+      if (c < (r >> 4) * 2 + 2) cp_async_16(smem + Sh::kRec + m * kRecT + tile_at<128>(r, c), rec + m * kRecT + r * 128 + c * 16);
     }
-    if (tid < 49) cp_async_16(smem + stage * Sh::kStage + Sh::kRec + kRecScal + tid * 16, rec + kRecScal + tid * 16);
-    rec += rec_step;
   };
   float* S = d.state + slot * d.slot_stride + static_cast<int64_t>(hv) * DK * DV + col + 16 * warp;
   float s[DK / 8][4];
   const bool zero = a.fresh && a.fresh[seq];
-  if (c0 < c1) load(0, c0);
+  if (c0 < c1) load_tokens(0, c0, rec);
+  cp_async_commit();
+  if (c0 < c1) load_matrices(rec);
   cp_async_commit();
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)
@@ -475,12 +516,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
 
   int stage = 0;
   for (int t0 = c0; t0 < c1; t0 += kC, stage ^= 1) {
-    if (t0 + kC < c1) load(stage ^ 1, t0 + kC);
+    cp_async_wait<1>();  // this chunk's tokens; its matrices may be on their way
+    __syncthreads();     // and every warp is done with the other stage
+    if (t0 + kC < c1) load_tokens(stage ^ 1, t0 + kC, rec + rec_step);
     cp_async_commit();
-    cp_async_wait<1>();
-    __syncthreads();
-    const uint32_t base = smem_u32(smem) + stage * Sh::kStage;
-    const float* f = reinterpret_cast<const float*>(smem + stage * Sh::kStage + Sh::kRec + kRecScal);
+    const uint32_t base = sm + stage * Sh::kStage, mat = sm + Sh::kRec;
+    const float* f = reinterpret_cast<const float*>(smem + stage * Sh::kStage + Sh::kF);
     // S0^T k_j and S0^T q_j of the chunk's tokens
     float r[8][4], o[8][4];
 #pragma unroll
@@ -496,7 +537,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
       for (int n = 0; n < 8; n += 2) {
         uint32_t b[4], q[4];
         const uint32_t at = tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi);
-        ldmatrix_x4(base + Sh::kK + at, b[0], b[1], b[2], b[3]);
+        ldmatrix_x4(base + at, b[0], b[1], b[2], b[3]);
         ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -507,6 +548,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
         }
       }
     }
+    cp_async_wait<1>();
+    __syncthreads();  // this chunk's matrices are here
     // R = v - exp(G) S0^T k; its two terms as A operands over the tokens
     uint32_t rh[4][4], rl[4][4];
 #pragma unroll
@@ -526,45 +569,89 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
         o[n + x][1] *= g.y;
         o[n + x][2] *= g.x;
         o[n + x][3] *= g.y;
-        split_bf16x2(y[0], y[1], rh[n / 2][2 * x], rl[n / 2][2 * x]);
-        split_bf16x2(y[2], y[3], rh[n / 2][2 * x + 1], rl[n / 2][2 * x + 1]);
       }
     }
-    // N = T R: token i needs tokens j <= i
+    // the two terms of a 16-token column block of x
+    auto split = [&](const float (&x)[8][4], int k, uint32_t (&h)[4], uint32_t (&l)[4]) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) split_bf16x2(x[2 * k + (y >> 1)][2 * (y & 1)], x[2 * k + (y >> 1)][2 * (y & 1) + 1], h[y], l[y]);
+    };
+    // (w0, w1) += rows (tokens) n*8 .. + 15 of the matrix, columns 16 k .. + 15, times block k of x
+    auto times = [&](float (&w0)[4], float (&w1)[4], int n, int k) {
+      uint32_t b[4], c[4];
+      const uint32_t at = tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi);
+      ldmatrix_x4(mat + at, b[0], b[1], b[2], b[3]);
+      ldmatrix_x4(mat + kRecT + at, c[0], c[1], c[2], c[3]);
+      mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
+      mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
+      mma_16816<true>(w0, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[0], b[1]);
+      mma_16816<true>(w1, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2], b[3]);
+      mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[0], c[1]);
+      mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[2], c[3]);
+    };
     float w[8][4];
 #pragma unroll
-    for (int n = 0; n < 8; n += 2) {
+    for (int n = 0; n < 8; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) w[n][x] = w[n + 1][x] = 0.f;
+      for (int x = 0; x < 4; ++x) w[n][x] = 0.f;
+    // N_0 = T_0 R_0
+    split(r, 0, rh[0], rl[0]);
+    split(r, 1, rh[1], rl[1]);
+    times(w[0], w[1], 0, 0);
+    times(w[2], w[3], 2, 0);
+    times(w[2], w[3], 2, 1);
+    // R_1 - B_10 N_0
+    split(w, 0, rh[0], rl[0]);
+    split(w, 1, rh[1], rl[1]);
 #pragma unroll
-      for (int k = 0; k <= n / 2; ++k) {
-        uint32_t b[4], c[4];
-        const uint32_t at = tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi);
-        ldmatrix_x4(base + Sh::kRec + at, b[0], b[1], b[2], b[3]);
-        ldmatrix_x4(base + Sh::kRec + kRecT + at, c[0], c[1], c[2], c[3]);
+    for (int n = 4; n < 8; n += 2) {
+      float p[2][4] = {};
+      times(p[0], p[1], n, 0);
+      times(p[0], p[1], n, 1);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          mma_16816<true>(w[n + x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
-          mma_16816<true>(w[n + x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2 * x], b[2 * x + 1]);
-          mma_16816<true>(w[n + x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[2 * x], c[2 * x + 1]);
-        }
-      }
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) r[n + x][y] -= p[x][y];
     }
+    // N_1 = T_1 (...)
+    split(r, 2, rh[2], rl[2]);
+    split(r, 3, rh[3], rl[3]);
+    times(w[4], w[5], 4, 2);
+    times(w[6], w[7], 6, 2);
+    times(w[6], w[7], 6, 3);
+    split(w, 2, rh[2], rl[2]);
+    split(w, 3, rh[3], rl[3]);
     // out += P N
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) split_bf16x2(w[2 * k + (x >> 1)][2 * (x & 1)], w[2 * k + (x >> 1)][2 * (x & 1) + 1], rh[k][x], rl[k][x]);
-#pragma unroll
       for (int n = 2 * k; n < 8; n += 2) {
         uint32_t b[4];
-        ldmatrix_x4(base + Sh::kRec + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[0], b[1], b[2], b[3]);
+        ldmatrix_x4(mat + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[0], b[1], b[2], b[3]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           mma_16816<true>(o[n + x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
           mma_16816<true>(o[n + x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2 * x], b[2 * x + 1]);
         }
       }
+    }
+    __syncthreads();  // every warp is done with the matrices
+    rec += rec_step;
+    if (t0 + kC < c1) load_matrices(rec);
+    cp_async_commit();
+    // the output's 16 columns of 64 tokens, turned in shared memory: in the place of the
+    // values, which no other warp reads
+#pragma unroll
+    for (int n = 0; n < 8; n += 2)
+      stmatrix_x4_trans(base + Sh::kVAt + tile_at<VR>(n * 8 + mtop * 8 + mrow, 2 * warp + mhi), pack16<true>(o[n][0], o[n][1]),
+                        pack16<true>(o[n][2], o[n][3]), pack16<true>(o[n + 1][0], o[n + 1][1]), pack16<true>(o[n + 1][2], o[n + 1][3]));
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = i * 16 + (lane >> 1);
+      if (t0 + t < c1)
+        *reinterpret_cast<uint4*>(d.out + (t0 + t) * d.out_stride + hv * DV + col + 16 * warp + (lane & 1) * 8) =
+            *reinterpret_cast<const uint4*>(smem + stage * Sh::kStage + Sh::kVAt + tile_at<VR>(t, 2 * warp + (lane & 1)));
     }
     // S = exp(G_64) S + k (exp(G_64 - G) n)^T
 #pragma unroll
@@ -581,7 +668,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t b[4];
-        ldmatrix_x4_trans(base + Sh::kK + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + mtop), b[0], b[1], b[2], b[3]);
+        ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
@@ -593,21 +680,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gated_delta_walk_kernel(const C
 #pragma unroll
         for (int y = 0; y < 4; ++y) s[n + x][y] = fmaf(s[n + x][y], end, p[x][y]);
     }
-    // the output's 16 columns of 64 tokens, turned in shared memory
-    uint8_t* ob = smem + Sh::kOut + warp * 2048;
-#pragma unroll
-    for (int n = 0; n < 8; n += 2)
-      stmatrix_x4_trans(smem_u32(ob) + (n * 8 + mtop * 8 + mrow) * 32 + mhi * 16, pack16<true>(o[n][0], o[n][1]),
-                        pack16<true>(o[n][2], o[n][3]), pack16<true>(o[n + 1][0], o[n + 1][1]), pack16<true>(o[n + 1][2], o[n + 1][3]));
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = i * 16 + (lane >> 1);
-      if (t0 + t < c1)
-        *reinterpret_cast<uint4*>(d.out + (t0 + t) * d.out_stride + hv * DV + col + 16 * warp + (lane & 1) * 8) =
-            *reinterpret_cast<const uint4*>(ob + t * 32 + (lane & 1) * 16);
-    }
-    __syncthreads();  // this stage may be filled again
   }
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)
@@ -683,12 +755,12 @@ int launch_prep(const ChunkArgs& a, cudaStream_t s) {
   return check_launch("d3_gated_delta_chunk");
 }
 
-template <int DK, int DV, int WARPS>
+template <int DK, int DV>
 int launch_walk(const ChunkArgs& a, cudaStream_t s) {
   static bool ready[64] = {};
-  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV, WARPS>, WalkShape<DK, WARPS>::kSmem, ready)) return rc;
-  launch_kernel(gated_delta_walk_kernel<DK, DV, WARPS>, dim3(DV / (16 * WARPS), a.d.value_heads, a.n), dim3(WARPS * 32),
-                WalkShape<DK, WARPS>::kSmem, s, a);
+  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV>, WalkShape<DK>::kSmem, ready)) return rc;
+  launch_kernel(gated_delta_walk_kernel<DK, DV>, dim3(DV / kWalkCols, a.d.value_heads, a.n), dim3(kWalkThreads),
+                WalkShape<DK>::kSmem, s, a);
   return check_launch("d3_gated_delta_chunk");
 }
 
@@ -696,10 +768,7 @@ template <int DK>
 int launch_chunk(const ChunkArgs& a, int dv, cudaStream_t s) {
   if (a.T > 0)
     if (int rc = launch_prep<DK>(a, s)) return rc;
-  if (dv == 64) return launch_walk<DK, 64, 4>(a, s);
-  // few sequences: twice the CTAs of half the columns
-  if (static_cast<int64_t>(a.n) * a.d.value_heads < sm_count()) return launch_walk<DK, 128, 4>(a, s);
-  return launch_walk<DK, 128, 8>(a, s);
+  return dv == 64 ? launch_walk<DK, 64>(a, s) : launch_walk<DK, 128>(a, s);
 }
 
 }  // namespace
