@@ -301,7 +301,7 @@ def call(name: str, *args) -> int:
 
     Invalid arguments surface as ValueError (the reference raises ValueError
     for shapes/strides, src/drama3/moe_input.py:47-62)."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc < 0:
         msg = (lib.d3_last_error_string() or b"").decode(errors="replace")

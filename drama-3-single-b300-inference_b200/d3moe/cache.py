@@ -8,8 +8,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import call
-from .attention import _index_ptr, _status_ptr
-from .ops import _stream
+from .attention import _index_ptr, _need_cuda, _status_ptr, _stream
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0, *,
@@ -20,13 +19,13 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_di
     and k / v). src and dst int32 [n] on the device; a negative number skips its
     pair, one past the pool too, with status set to D3_STATUS_BAD_ROW. No page
     may be both copied from and copied to in one call, nor copied to twice."""
-    if not pool.is_cuda:
-        raise ValueError("d3moe operators take CUDA tensors; there is no CPU path")
+    dev = pool.get_device()
+    _need_cuda(dev)
     shape, strides = pool.shape, pool.stride()
-    if not 0 <= page_dim < pool.dim():
+    if not 0 <= page_dim < len(shape):
         raise ValueError("page_dim must be an axis of pool")
     elements = 1
-    for i in range(pool.dim() - 1, page_dim, -1):
+    for i in range(len(shape) - 1, page_dim, -1):
         if shape[i] != 1 and strides[i] != elements:
             raise ValueError("the axes behind page_dim must be contiguous")
         elements *= shape[i]
@@ -39,7 +38,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_di
         elif strides[i] != planes * plane_stride:
             raise ValueError("the axes before page_dim must step evenly")
         planes *= shape[i]
-    n, dev, size = src.numel(), pool.device, pool.element_size()
+    n, size = src.numel(), pool.element_size()
     call("d3_copy_pages", pool.data_ptr(), planes, plane_stride * size, shape[page_dim],
          strides[page_dim] * size, elements * size, _index_ptr(src, n, dev, "src"),
          _index_ptr(dst, n, dev, "dst"), n, _status_ptr(status, dev), _stream(dev))
