@@ -1,8 +1,9 @@
-"""Builds libd3moe.so (every CUDA source under csrc/) for sm_100a with nvcc.
+"""Builds libd3moe.so (every CUDA source under csrc/) for sm_100a with nvcc, and the
+CPython binding _d3native.so (csrc/binding/) with g++.
 
-The library is written in-tree next to the Python package
-(d3moe/_lib/libd3moe.so) so that it travels with the source tree; it is
-rebuilt only when a source or header is newer than the library.
+The libraries are written in-tree next to the Python package (d3moe/_lib/) so
+that they travel with the source tree; they are rebuilt only when a source or
+header is newer than they are.
 
 Usage: python build.py [--force] [--verbose]
 """
@@ -22,6 +23,8 @@ OUT_DIR = HERE / "d3moe" / "_lib"
 LIB = OUT_DIR / "libd3moe.so"
 # test-only library (csrc/selftest/): failure-path probes kept out of the product
 SELFTEST_LIB = OUT_DIR / "libd3moe_selftest.so"
+# CPython binding of the operators whose host time counts (csrc/binding/)
+NATIVE_LIB = OUT_DIR / "_d3native.so"
 INCLUDE = HERE.parent / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,9 +52,10 @@ def sources() -> list[Path]:
 
 
 def needs_build() -> bool:
-    if not LIB.exists() or not SELFTEST_LIB.exists():
+    built = (LIB, SELFTEST_LIB, NATIVE_LIB)
+    if not all(p.exists() for p in built):
         return True
-    lib_time = min(LIB.stat().st_mtime, SELFTEST_LIB.stat().st_mtime)
+    lib_time = min(p.stat().st_mtime for p in built)
     deps = list(CSRC.rglob("*")) + list(INCLUDE.glob("*.h")) + [Path(__file__)]
     return any(p.stat().st_mtime > lib_time for p in deps if p.is_file())
 
@@ -72,6 +76,30 @@ def _link(cc: str, srcs: list[Path], out: Path, objdir: Path, verbose: bool) -> 
     os.replace(tmp, out)
 
 
+def _link_binding(out: Path, verbose: bool) -> None:
+    """The CPython binding, against torch's headers and libraries."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cxx = os.environ.get("CXX") or shutil.which("g++")
+    if not cxx:
+        raise RuntimeError("g++ not found; it compiles the CPython binding")
+    cuda = Path(nvcc()).resolve().parents[1]
+    include = [INCLUDE, root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               cuda / "include", Path(sysconfig.get_paths()["include"])]
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-I{p}" for p in include], *map(str, sorted((CSRC / "binding").glob("*.cpp"))), "-o", str(tmp),
+           f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, out)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
@@ -81,6 +109,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     cc = nvcc()
     _link(cc, sources(), LIB, objdir, verbose)
     _link(cc, sorted((CSRC / "selftest").glob("*.cu")), SELFTEST_LIB, objdir, verbose)
+    _link_binding(NATIVE_LIB, verbose)
     return LIB
 
 

@@ -273,6 +273,37 @@ class D3Error(RuntimeError):
 
 
 _lib = None
+_native = None
+
+# what the CPython binding calls, in the order of its bind()
+_NATIVE_CALLS = ("d3_kv_append", "d3_copy_pages", "d3_paged_attention", "d3_paged_attention_workspace_size",
+                 "d3_gated_delta_step", "d3_gated_delta_chunk", "d3_gated_delta_chunk_workspace_size",
+                 "d3_last_error_string")
+
+
+def native():
+    """The CPython binding (csrc/binding/), connected to the loaded library:
+    the operators a decode step calls many times reach the C ABI through it."""
+    global _native
+    if _native is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (the binding uses its libraries)
+
+        lib = load()
+        p = _HERE / "_lib" / "_d3native.so"
+        if not p.exists():
+            raise ImportError(
+                f"_d3native.so not found at {p}; build it with "
+                "`python drama-3-single-b300-inference_b200/build.py`"
+            )
+        loader = importlib.machinery.ExtensionFileLoader("_d3native", str(p))
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_d3native", loader))
+        loader.exec_module(mod)
+        mod.bind(D3Error, *(ctypes.cast(getattr(lib, n), _c_void_p).value for n in _NATIVE_CALLS))
+        _native = mod
+    return _native
 
 
 def load(path: Path | None = None) -> ctypes.CDLL:
