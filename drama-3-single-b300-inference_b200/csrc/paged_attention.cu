@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool QBF16 = DT != D3_DTYPE_F16;
   constexpr int ROWS = Sh::kRows, LANES = D / 4, GROUPS = kAttnThreads / LANES;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   float4* acc = reinterpret_cast<float4*>(smem);                       // [GROUPS][LANES]
   float* fac = reinterpret_cast<float*>(smem) + kAttnThreads * 4;      // [a.grid] maximum, then weight
   float* red = fac + a.grid;                                           // [2][warps]
