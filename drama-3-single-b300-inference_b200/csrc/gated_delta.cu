@@ -7,7 +7,9 @@
 // so the state is read once and written once.
 //
 // One CTA per (sequence, value head, 32 value columns): thread (row group,
-// column quad) keeps rows r, r + 16, ... of 4 columns in registers.
+// column quad) keeps consecutive rows of 4 columns in registers. Everything a CTA
+// reads is asked for at once, and the sums over the rows (with those of q.q, k.k and
+// k.q, which give the norms) meet in one exchange.
 //
 // Packed prompts go in chunks of 64 tokens. With G_i the sum of g up to token i
 // of the chunk, k_i and q_i the normalised keys and scaled queries, and S0 the state
@@ -73,97 +75,100 @@ __device__ __forceinline__ int delta_slot(const DeltaArgs& a, int i) {
 template <int DK, int DV>
 __global__ void __launch_bounds__(kDeltaThreads)
     gated_delta_step_kernel(const DeltaArgs a) {
-  constexpr int R = DK / 16;  // state rows of a thread
-  __shared__ float s_q[DK], s_k[DK];
-  __shared__ float s_part[2][4][kDeltaCols];
-  __shared__ float s_dot[3][4];
+  constexpr int R = DK / 16;  // state rows of a thread: R * (row group) ...
+  __shared__ float4 s_part[4][2][kDeltaCols / 4];
+  __shared__ float s_dot[4][3];
   pdl_enter();
   const int seq = blockIdx.z, h = blockIdx.y, c0 = blockIdx.x * kDeltaCols;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cq = (tid & 7) * 4, rg = tid >> 3;
   const int hk = h / a.rep;
-  const int t = seq;
   const int slot = delta_slot(a, seq);
+  __nv_bfloat16* out = a.out + seq * a.out_stride + h * DV + c0;
   if (slot < 0) {
-    if (tid < kDeltaCols) a.out[t * a.out_stride + h * DV + c0 + tid] = __float2bfloat16_rn(0.f);
+    if (tid < kDeltaCols / 4) *reinterpret_cast<uint2*>(out + tid * 4) = make_uint2(0, 0);
     return;
   }
-  float* S = a.state + slot * a.slot_stride + static_cast<int64_t>(h) * DK * DV + c0 + cq;
-  float s[R][4];
+  float* S = a.state + slot * a.slot_stride + static_cast<int64_t>(h) * DK * DV + (rg * R) * DV + c0 + cq;
+  float4 s[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) s[r] = *reinterpret_cast<const float4*>(S + r * DV);
+  uint32_t qw[R / 2], kw[R / 2];
+  const __nv_bfloat16 *qp = a.q + seq * a.q_stride + hk * DK + rg * R, *kp = a.k + seq * a.k_stride + hk * DK + rg * R;
+  if constexpr (R == 8) {
+    const uint4 x = *reinterpret_cast<const uint4*>(qp), y = *reinterpret_cast<const uint4*>(kp);
+    qw[0] = x.x; qw[1] = x.y; qw[2] = x.z; qw[3] = x.w;
+    kw[0] = y.x; kw[1] = y.y; kw[2] = y.z; kw[3] = y.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(qp), y = *reinterpret_cast<const uint2*>(kp);
+    qw[0] = x.x; qw[1] = x.y;
+    kw[0] = y.x; kw[1] = y.y;
+  }
+  const uint2 vw = *reinterpret_cast<const uint2*>(a.v + seq * a.v_stride + h * DV + c0 + cq);
+  const float g = __ldg(a.g + seq * a.g_stride + h), beta = __ldg(a.beta + seq * a.beta_stride + h);
+  float k[R], pa[4] = {}, pc[4] = {}, qq = 0.f, kk = 0.f, qk = 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float4 x = *reinterpret_cast<const float4*>(S + (rg + 16 * r) * DV);
-    s[r][0] = x.x; s[r][1] = x.y; s[r][2] = x.z; s[r][3] = x.w;
+    k[r] = __uint_as_float(r & 1 ? kw[r / 2] & 0xffff0000u : kw[r / 2] << 16);
+    const float q = __uint_as_float(r & 1 ? qw[r / 2] & 0xffff0000u : qw[r / 2] << 16);
+    qq = fmaf(q, q, qq);
+    kk = fmaf(k[r], k[r], kk);
+    qk = fmaf(q, k[r], qk);
+    pa[0] = fmaf(s[r].x, k[r], pa[0]); pa[1] = fmaf(s[r].y, k[r], pa[1]);
+    pa[2] = fmaf(s[r].z, k[r], pa[2]); pa[3] = fmaf(s[r].w, k[r], pa[3]);
+    pc[0] = fmaf(s[r].x, q, pc[0]); pc[1] = fmaf(s[r].y, q, pc[1]);
+    pc[2] = fmaf(s[r].z, q, pc[2]); pc[3] = fmaf(s[r].w, q, pc[3]);
   }
-  float qv = 0.f, kv = 0.f;
-  if (tid < DK) {
-    qv = __bfloat162float(a.q[t * a.q_stride + hk * DK + tid]);
-    kv = __bfloat162float(a.k[t * a.k_stride + hk * DK + tid]);
-    s_q[tid] = qv;
-    s_k[tid] = kv;
-  }
-  float qq = qv * qv, kk = kv * kv, qk = qv * kv;
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
+  for (int x = 8; x <= 16; x <<= 1) {  // the 4 row groups of the warp
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      pa[j] += __shfl_xor_sync(0xffffffffu, pa[j], x);
+      pc[j] += __shfl_xor_sync(0xffffffffu, pc[j], x);
+    }
     qq += __shfl_xor_sync(0xffffffffu, qq, x);
     kk += __shfl_xor_sync(0xffffffffu, kk, x);
     qk += __shfl_xor_sync(0xffffffffu, qk, x);
   }
-  if (lane == 0) {
-    s_dot[0][warp] = qq;
-    s_dot[1][warp] = kk;
-    s_dot[2][warp] = qk;
+  if (lane < 8) {
+    s_part[warp][0][lane] = make_float4(pa[0], pa[1], pa[2], pa[3]);
+    s_part[warp][1][lane] = make_float4(pc[0], pc[1], pc[2], pc[3]);
+    if (lane == 0) {
+      s_dot[warp][0] = qq;
+      s_dot[warp][1] = kk;
+      s_dot[warp][2] = qk;
+    }
   }
   __syncthreads();
-  qq = s_dot[0][0] + s_dot[0][1] + s_dot[0][2] + s_dot[0][3];
-  kk = s_dot[1][0] + s_dot[1][1] + s_dot[1][2] + s_dot[1][3];
-  qk = s_dot[2][0] + s_dot[2][1] + s_dot[2][2] + s_dot[2][3];
+  qq = kk = qk = 0.f;
+  float xa[4] = {}, xc[4] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    qq += s_dot[w][0];
+    kk += s_dot[w][1];
+    qk += s_dot[w][2];
+    const float4 x = s_part[w][0][tid & 7], y = s_part[w][1][tid & 7];
+    xa[0] += x.x; xa[1] += x.y; xa[2] += x.z; xa[3] += x.w;
+    xc[0] += y.x; xc[1] += y.y; xc[2] += y.z; xc[3] += y.w;
+  }
   const float rq = a.scale * (a.l2norm ? rsqrtf(qq + a.eps) : 1.f);
   const float rk = a.l2norm ? rsqrtf(kk + a.eps) : 1.f;
-  float pa[4] = {}, pc[4] = {};
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float kr = s_k[rg + 16 * r], qr = s_q[rg + 16 * r];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      pa[j] = fmaf(s[r][j], kr, pa[j]);
-      pc[j] = fmaf(s[r][j], qr, pc[j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int x = 8; x <= 16; x <<= 1) {
-      pa[j] += __shfl_xor_sync(0xffffffffu, pa[j], x);
-      pc[j] += __shfl_xor_sync(0xffffffffu, pc[j], x);
-    }
-    if (lane < 8) {
-      s_part[0][warp][cq + j] = pa[j];
-      s_part[1][warp][cq + j] = pc[j];
-    }
-  }
-  __syncthreads();
-  const float eg = expf(__ldg(a.g + t * a.g_stride + h)), be = __ldg(a.beta + t * a.beta_stride + h);
+  const float eg = expf(g);
+  const float v[4] = {__uint_as_float(vw.x << 16), __uint_as_float(vw.x & 0xffff0000u), __uint_as_float(vw.y << 16),
+                      __uint_as_float(vw.y & 0xffff0000u)};
   float d[4], o[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float xa = s_part[0][0][cq + j] + s_part[0][1][cq + j] + s_part[0][2][cq + j] + s_part[0][3][cq + j];
-    const float xc = s_part[1][0][cq + j] + s_part[1][1][cq + j] + s_part[1][2][cq + j] + s_part[1][3][cq + j];
-    d[j] = be * (__bfloat162float(a.v[t * a.v_stride + h * DV + c0 + cq + j]) - eg * rk * xa);
-    o[j] = rq * (eg * xc + qk * rk * d[j]);
+    d[j] = beta * (v[j] - eg * rk * xa[j]);
+    o[j] = rq * (eg * xc[j] + qk * rk * d[j]);
   }
-  if (rg == 0)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a.out[t * a.out_stride + h * DV + c0 + cq + j] = __float2bfloat16_rn(o[j]);
+  if (rg == 0) *reinterpret_cast<uint2*>(out + cq) = make_uint2(pack16<true>(o[0], o[1]), pack16<true>(o[2], o[3]));
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const float kr = s_k[rg + 16 * r] * rk;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[r][j] = fmaf(kr, d[j], eg * s[r][j]);
+    const float kr = k[r] * rk;
+    *reinterpret_cast<float4*>(S + r * DV) = make_float4(fmaf(kr, d[0], eg * s[r].x), fmaf(kr, d[1], eg * s[r].y),
+                                                         fmaf(kr, d[2], eg * s[r].z), fmaf(kr, d[3], eg * s[r].w));
   }
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    *reinterpret_cast<float4*>(S + (rg + 16 * r) * DV) = make_float4(s[r][0], s[r][1], s[r][2], s[r][3]);
 }
 
 
