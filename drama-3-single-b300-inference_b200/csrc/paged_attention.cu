@@ -16,13 +16,14 @@
 //
 // Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
 // tile, loads them with cp.async into its own ring of shared-memory slots (keys
-// and values of a tile are two slots; no barrier between warps), and works with mma.sync m16n8k16: queries are
-// the 16 rows of A, keys the columns of B for the logits, and the probabilities
-// go back in as A from the registers that hold them (the accumulator layout is
-// the A layout). tcgen05 has nothing to add here: its 128-row tile would be 1/16
-// used. With up to 8 query heads per key head only rows 0-7 of A are needed, and
-// rows 8-15 carry, for bf16, the part of each probability that its rounding
-// to bf16 lost: the products are then exact to 2^-17 at no cost.
+// and values of a tile are two slots; no barrier between warps), and works with
+// mma.sync m16n8k16 on transposes: the keys are the 16 rows of A and 8 query heads the
+// columns of B for the logits, and V^T is A for the output, so with up to 8 heads per
+// key head no part of a product is idle; the probabilities turn into B operands by
+// one movmatrix each. tcgen05 has nothing to add: its tile of 128 rows of keys per
+// instruction would need 8 columns at most, and the operands' way through shared
+// memory is the same. bf16 probabilities go in two terms (2^-17), so the output is
+// rounded once, at its end.
 //
 // An e4m3 cache is widened to f16 in registers (exact). Its queries are scaled by
 // a power of two per row into f16's range (exact for every element within 2^-14
@@ -35,7 +36,6 @@ namespace {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kMaxSmem = 113 * 1024;  // of one CTA: two share an SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -66,12 +66,16 @@ template <int DT, int D, bool WIDE>
 struct AttnShape {
   static constexpr int kElem = DT == D3_DTYPE_E4M3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  // keys of one warp and tile: a slot of the ring holds up to 8 KB
-  static constexpr int kNK = 8192 / kRowBytes < 32 ? 8192 / kRowBytes : 32;
+  // CTAs that share an SM, and what of its shared memory one may take
+  static constexpr int kCtas = D == 256 ? 2 : 3;
+  static constexpr int kMaxSmem = (D == 256 ? 113 : 75) * 1024;
+  // keys of one warp and tile, 16 or 32: a slot of the ring holds 8 KB for 256 columns, up to 4 KB else
+  static constexpr int kNK = kRowBytes == 256 || kRowBytes == 512 ? (D == 256 && kElem == 1 ? 32 : 16) : 32;
   static constexpr int kTile = kNK * kAttnWarps;
   static constexpr int kRows = WIDE ? 16 : 8;
   static constexpr int kHalf = kNK * kRowBytes;  // bytes of a slot
-  static constexpr int kAhead = (24576 / kHalf - 1) / 2 < 4 ? (24576 / kHalf - 1) / 2 : 4;  // tiles loaded ahead
+  static constexpr int kFit = ((D == 256 ? 24576 : 16384) / kHalf - 1) / 2;
+  static constexpr int kAhead = kFit < 4 ? kFit : 4;  // tiles loaded ahead
   static constexpr int kSlots = 2 * kAhead + 1;
   static constexpr int kWarpRing = kSlots * kHalf;
   static constexpr int kRing = kAttnWarps * kWarpRing;
@@ -80,7 +84,7 @@ struct AttnShape {
   static constexpr int kQPieces = (kRows * D * 2 / 16 + kAttnThreads - 1) / kAttnThreads;  // of one thread
   static constexpr int kStat = kAttnWarps * 32 * 4 + 64;
   // 8 output rows of kJoinWarps warps at a time are added up in shared memory
-  static constexpr int kJoinPitch = D + (D == 256 && WIDE ? 4 : kElem == 1 ? 16 : 8);  // floats, padded likewise
+  static constexpr int kJoinPitch = D + 4;     // floats, padded likewise
   static constexpr int kJoinFit = (kMaxSmem - kRing - kQ - kStat) / (8 * kJoinPitch * 4);
   static constexpr int kJoinWarps = kJoinFit >= 4 ? 4 : kJoinFit >= 2 ? 2 : 1;
   static constexpr int kJoin = kJoinWarps * 8 * kJoinPitch * 4;
@@ -182,13 +186,12 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int d
 }
 
 template <int DT, int D, bool WIDE>
-__global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas)) paged_attention_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool BF16 = DT == D3_DTYPE_BF16;        // type of the matrix products
   constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
-  constexpr bool SPLIT = BF16 && !WIDE;             // rows 8-15 carry the rounding's rest
   constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kSlots, P = Sh::kAhead, ROWS = Sh::kRows;
-  constexpr int KS = D / 16, NT = NK / 8, DT8 = D / 8;
+  constexpr int KS = D / 16, MT = NK / 16, NH = ROWS / 8;
   constexpr int PIECES = RB / 16, JW = Sh::kJoinWarps, JP = Sh::kJoinPitch;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* join = reinterpret_cast<float*>(smem + Sh::kRing);
@@ -311,9 +314,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
   place_q();
   __syncthreads();
 
-  uint32_t qf[KS][WIDE ? 4 : 2];
-  float o[DT8][4], m[WIDE ? 2 : 1], l[WIDE ? 2 : 1];
-  float lg[WIDE ? 2 : 1];  // logit in units of log2 per product
+  uint32_t qf[KS][NH][2];  // queries as B operands: a column per head
+  float o[KS][NH][4];      // 16 columns of V by 8 heads each
+  float m[NH][2], l[NH][2];  // of heads 2 t4 and 2 t4 + 1
+  float lg[NH][2];         // their logits in units of log2, per product
   bool opened = false, whole = false;
   int seg_slot = 0, use = 0;
   bool more = true;
@@ -326,14 +330,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
       whole = cur.tile == 0;
       seg_slot = begun;
 #pragma unroll
-      for (int d = 0; d < DT8; ++d)
+      for (int h = 0; h < NH; ++h) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[d][x] = 0.f;
+        for (int d = 0; d < KS; ++d)
 #pragma unroll
-      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
-        m[w] = -INFINITY;
-        l[w] = 0.f;
-        const uint8_t* row = qs + (quad + 8 * w) * Sh::kQPitch;
+          for (int x = 0; x < 4; ++x) o[d][h][x] = 0.f;
+        m[h][0] = m[h][1] = -INFINITY;
+        l[h][0] = l[h][1] = 0.f;
+        const uint8_t* row = qs + (quad + 8 * h) * Sh::kQPitch;
         float ks = a.scale * kLog2e;
         if constexpr (DT == D3_DTYPE_E4M3) {
           // the row's largest element decides its power of two
@@ -350,21 +354,24 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
           if (top > 0.f && isfinite(top)) frexpf(top, &e);
           e = max(-100, min(100, e));  // 2^-e and 2^e both exist
           const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          // k index 2 t4 + {0, 1, 8, 9} stands for column 4 t4 + {0, 1, 2, 3}, as in the keys below
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             const uint2 y = *reinterpret_cast<const uint2*>(row + 32 * s + 8 * t4);
-            qf[s][w] = pack16<false>(__uint_as_float(y.x << 16) * down, __uint_as_float(y.x & 0xffff0000u) * down);
-            qf[s][WIDE ? 2 + w : 1] = pack16<false>(__uint_as_float(y.y << 16) * down, __uint_as_float(y.y & 0xffff0000u) * down);
+            qf[s][h][0] = pack16<false>(__uint_as_float(y.x << 16) * down, __uint_as_float(y.x & 0xffff0000u) * down);
+            qf[s][h][1] = pack16<false>(__uint_as_float(y.y << 16) * down, __uint_as_float(y.y & 0xffff0000u) * down);
           }
           ks *= (a.k_scale ? __ldg(a.k_scale + head) : 1.0f) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         } else {
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
-            qf[s][w] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4);
-            qf[s][WIDE ? 2 + w : 1] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4 + 16);
+            qf[s][h][0] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4);
+            qf[s][h][1] = *reinterpret_cast<const uint32_t*>(row + 32 * s + 4 * t4 + 16);
           }
         }
-        lg[w] = ks;
+        // from the lanes that hold the head's column to those that hold its logits
+        lg[h][0] = __shfl_sync(0xffffffffu, ks, 8 * t4);
+        lg[h][1] = __shfl_sync(0xffffffffu, ks, 8 * t4 + 4);
       }
     }
     // the next loads go out before this tile's work
@@ -373,89 +380,96 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
     __syncwarp();
     const uint32_t ks = ring + use * Sh::kHalf;
     use = use + 1 == S ? 0 : use + 1;
-    float s[NT][4];
+    // logits: the keys are A's rows, the queries B's columns
+    float s[MT][NH][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int r = 0; r < MT; ++r)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
-    // logits: rows of K are the columns of B
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[r][h][x] = 0.f;
     const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
     if constexpr (DT == D3_DTYPE_E4M3) {
 #pragma unroll
       for (int c = 0; c < KS; c += 2)  // 16 bytes of a row are one k step
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
+        for (int r = 0; r < MT; ++r) {
           uint32_t b[4];
-          ldmatrix_x4(ks + tile_at<RB>(n * 8 + mtop * 8 + mrow, c + mhi), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4(ks + tile_at<RB>(r * 16 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
-          for (int y = 0; y < 2; ++y)    // k step
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t w0 = b[2 * y], w1 = b[2 * y + 1];  // keys 0-7, keys 8-15
+            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w0)), a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w1));
+            const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(w0 >> 16)), a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(w1 >> 16));
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {  // 8 keys
-              const uint32_t w = b[2 * x + y];
-              const uint32_t b0 = e4m3x2_to_f16x2(static_cast<uint16_t>(w)), b1 = e4m3x2_to_f16x2(static_cast<uint16_t>(w >> 16));
-              if constexpr (WIDE) mma_16816<false>(s[n + x], qf[c + y][0], qf[c + y][1], qf[c + y][2], qf[c + y][3], b0, b1);
-              else mma_16816<false>(s[n + x], qf[c + y][0], 0u, qf[c + y][1], 0u, b0, b1);
-            }
+            for (int h = 0; h < NH; ++h) mma_16816<false>(s[r][h], a0, a1, a2, a3, qf[c + y][h][0], qf[c + y][h][1]);
+          }
         }
     } else {
 #pragma unroll
       for (int c = 0; c < KS; ++c)
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
+        for (int r = 0; r < MT; ++r) {
           uint32_t b[4];
-          ldmatrix_x4(ks + tile_at<RB>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4(ks + tile_at<RB>(r * 16 + mhi * 8 + mrow, 2 * c + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if constexpr (WIDE) mma_16816<BF16>(s[n + x], qf[c][0], qf[c][1], qf[c][2], qf[c][3], b[2 * x], b[2 * x + 1]);
-            else mma_16816<BF16>(s[n + x], qf[c][0], 0u, qf[c][1], 0u, b[2 * x], b[2 * x + 1]);
-          }
+          for (int h = 0; h < NH; ++h) mma_16816<BF16>(s[r][h], b[0], b[1], b[2], b[3], qf[c][h][0], qf[c][h][1]);
         }
     }
     // keys past the end take no part
     const int left = cur.len - (cur.begin + cur.tile * Sh::kTile + warp * NK);
-    uint32_t pf[NT][2];  // probabilities as A operands: [8 keys][rows 0-7, rows 8-15]
+    uint32_t pb[MT][NH][2], pl[MT][NH][2];  // probabilities as B operands; what their rounding lost
 #pragma unroll
-    for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
-      float top = -INFINITY;
+    for (int h = 0; h < NH; ++h) {
+      float mn[2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int x = 0; x < 2; ++x) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < MT; ++r)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float& z = s[r][h][2 * y + x];
+            z = r * 16 + y * 8 + quad < left ? z * lg[h][x] : -INFINITY;
+            top = fmaxf(top, z);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        mn[x] = fmaxf(m[h][x], top);
+      }
+      if (__any_sync(0xffffffffu, mn[0] > m[h][0] || mn[1] > m[h][1])) {  // some head has a new maximum: rescale
+        float c[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float& y = s[n][2 * w + x];
-          y = n * 8 + 2 * t4 + x < left ? y * lg[w] : -INFINITY;
-          top = fmaxf(top, y);
+          c[x] = exp2f(m[h][x] - (mn[x] == -INFINITY ? 0.f : mn[x]));
+          l[h][x] *= c[x];
         }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(m[w], top);
-      if (__any_sync(0xffffffffu, mn > m[w])) {  // some row has a new maximum: rescale what it has
-        const float c = exp2f(m[w] - (mn == -INFINITY ? 0.f : mn));
-        l[w] *= c;
 #pragma unroll
-        for (int d = 0; d < DT8; ++d) {
-          o[d][2 * w] *= c;
-          o[d][2 * w + 1] *= c;
-          if constexpr (SPLIT) {
-            o[d][2] *= c;
-            o[d][3] *= c;
-          }
+        for (int d = 0; d < KS; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[d][h][x] *= c[x & 1];
+      }
+      float base[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[h][x] = mn[x];
+        base[x] = mn[x] == -INFINITY ? 0.f : mn[x];  // no key yet, or only logits of -inf
+      }
+#pragma unroll
+      for (int r = 0; r < MT; ++r)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float p0 = exp2f(s[r][h][2 * y] - base[0]), p1 = exp2f(s[r][h][2 * y + 1] - base[1]);
+          l[h][0] += p0;
+          l[h][1] += p1;
+          const uint32_t hi = pack16<BF16>(p0, p1);
+          pb[r][h][y] = movmatrix_trans(hi);  // a key's row of heads becomes a head's column of keys
+          if constexpr (BF16)
+            pl[r][h][y] = movmatrix_trans(pack16<true>(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u)));
         }
-      }
-      m[w] = mn;
-      const float base = mn == -INFINITY ? 0.f : mn;  // no key yet, or only logits of -inf
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float p0 = exp2f(s[n][2 * w] - base), p1 = exp2f(s[n][2 * w + 1] - base);
-        l[w] += p0 + p1;
-        const uint32_t hi = pack16<BF16>(p0, p1);
-        pf[n][w] = hi;
-        if constexpr (SPLIT)
-          pf[n][1] = pack16<true>(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
-        else if constexpr (!WIDE)
-          pf[n][1] = 0u;
-      }
     }
-    // out += P V
+    // out^T += V^T P^T
     __syncwarp();  // every lane has read the keys' slot: it may be filled again
     load_values();
     cp_async_wait<S - 1>();
@@ -464,33 +478,36 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
     use = use + 1 == S ? 0 : use + 1;
     if constexpr (DT == D3_DTYPE_E4M3) {
 #pragma unroll
-      for (int n = 0; n < NT; n += 2)
+      for (int r = 0; r < MT; ++r)
 #pragma unroll
-        for (int c = 0; c < D / 16; c += 2) {
+        for (int c = 0; c < KS; c += 2) {
           uint32_t b[4];
-          ldmatrix_x4_trans(vs + tile_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
+          ldmatrix_x4_trans(vs + tile_at<RB>(r * 16 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            // a 16-bit unit holds two neighbouring columns of a key: even and
-            // odd columns go to two products
+            // a 16-bit unit holds two neighbouring columns of a key: the even ones
+            // become rows 0-7 of A, the odd ones rows 8-15
             const uint32_t w0 = b[2 * y], w1 = b[2 * y + 1];
-            const uint32_t e0 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0020)));
-            const uint32_t e1 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0020)));
-            const uint32_t d0 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0031)));
-            const uint32_t d1 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0031)));
-            mma_16816<false>(o[2 * (c + y)], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], e0, e1);
-            mma_16816<false>(o[2 * (c + y) + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], d0, d1);
+            const uint32_t a0 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0020)));
+            const uint32_t a1 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w0, 0, 0x0031)));
+            const uint32_t a2 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0020)));
+            const uint32_t a3 = e4m3x2_to_f16x2(static_cast<uint16_t>(__byte_perm(w1, 0, 0x0031)));
+#pragma unroll
+            for (int h = 0; h < NH; ++h) mma_16816<false>(o[c + y][h], a0, a1, a2, a3, pb[r][h][0], pb[r][h][1]);
           }
         }
     } else {
 #pragma unroll
-      for (int n = 0; n < NT; n += 2)
+      for (int r = 0; r < MT; ++r)
 #pragma unroll
-        for (int c = 0; c < DT8; c += 2) {
+        for (int c = 0; c < KS; ++c) {
           uint32_t b[4];
-          ldmatrix_x4_trans(vs + tile_at<RB>(n * 8 + mhi * 8 + mrow, c + mtop), b[0], b[1], b[2], b[3]);
-          mma_16816<BF16>(o[c], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[0], b[1]);
-          mma_16816<BF16>(o[c + 1], pf[n][0], pf[n][1], pf[n + 1][0], pf[n + 1][1], b[2], b[3]);
+          ldmatrix_x4_trans(vs + tile_at<RB>(r * 16 + mtop * 8 + mrow, 2 * c + mhi), b[0], b[1], b[2], b[3]);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            mma_16816<BF16>(o[c][h], b[0], b[1], b[2], b[3], pb[r][h][0], pb[r][h][1]);
+            if constexpr (BF16) mma_16816<true>(o[c][h], b[0], b[1], b[2], b[3], pl[r][h][0], pl[r][h][1]);
+          }
         }
     }
     __syncwarp();  // the same for the values
@@ -504,14 +521,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
       opened = false;
       if (more) fetch_q(nxt);
 #pragma unroll
-      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
-        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
-        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-        if (t4 == 0) {
-          stat[warp * 32 + quad + 8 * w] = m[w];
-          stat[warp * 32 + 16 + quad + 8 * w] = l[w];
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          l[h][x] += __shfl_xor_sync(0xffffffffu, l[h][x], 4);
+          l[h][x] += __shfl_xor_sync(0xffffffffu, l[h][x], 8);
+          l[h][x] += __shfl_xor_sync(0xffffffffu, l[h][x], 16);
+          if (quad == 0) {
+            stat[warp * 32 + 8 * h + 2 * t4 + x] = m[h][x];
+            stat[warp * 32 + 16 + 8 * h + 2 * t4 + x] = l[h][x];
+          }
         }
-      }
       __syncthreads();
       whole = whole && last;
       float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
@@ -519,37 +539,35 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attention_kernel(const 
       // each warp scales its rows to the common maximum; JW at a time they are
       // added into JW buffers, in the order of the warps
 #pragma unroll
-      for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+      for (int w = 0; w < NH; ++w) {
         if (w) __syncthreads();
 #pragma unroll 1
         for (int round = 0; round < kAttnWarps / JW; ++round) {
           if (warp / JW == round) {
-            float top = -INFINITY;
+            float f[2];
 #pragma unroll
-            for (int x = 0; x < kAttnWarps; ++x) top = fmaxf(top, stat[x * 32 + quad + 8 * w]);
-            const float f = exp2f(m[w] - (top == -INFINITY ? 0.f : top));
-            float* row = join + ((warp % JW) * 8 + quad) * JP;
-            if constexpr (DT == D3_DTYPE_E4M3) {
+            for (int x = 0; x < 2; ++x) {
+              float top = -INFINITY;
 #pragma unroll
-              for (int d = 0; d < DT8; d += 2) {
-                float4* at = reinterpret_cast<float4*>(row + d * 8 + 4 * t4);
-                const float4 was = round ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                *at = make_float4(fmaf(o[d][2 * w], f, was.x), fmaf(o[d + 1][2 * w], f, was.y),
-                                  fmaf(o[d][2 * w + 1], f, was.z), fmaf(o[d + 1][2 * w + 1], f, was.w));
-              }
-            } else {
-#pragma unroll
-              for (int d = 0; d < DT8; ++d) {
-                float x0 = o[d][2 * w], x1 = o[d][2 * w + 1];
-                if constexpr (SPLIT) {
-                  x0 += o[d][2];
-                  x1 += o[d][3];
-                }
-                float2* at = reinterpret_cast<float2*>(row + d * 8 + 2 * t4);
-                const float2 was = round ? *at : make_float2(0.f, 0.f);
-                *at = make_float2(fmaf(x0, f, was.x), fmaf(x1, f, was.y));
-              }
+              for (int y = 0; y < kAttnWarps; ++y) top = fmaxf(top, stat[y * 32 + 8 * w + 2 * t4 + x]);
+              f[x] = exp2f(m[w][x] - (top == -INFINITY ? 0.f : top));
             }
+            float* row = join + ((warp % JW) * 8 + 2 * t4) * JP;
+#pragma unroll
+            for (int d = 0; d < KS; ++d)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float y0 = o[d][w][x], y1 = o[d][w][2 + x];  // rows quad, quad + 8
+                if constexpr (DT == D3_DTYPE_E4M3) {
+                  float2* at = reinterpret_cast<float2*>(row + x * JP + d * 16 + 2 * quad);
+                  const float2 was = round ? *at : make_float2(0.f, 0.f);
+                  *at = make_float2(fmaf(y0, f[x], was.x), fmaf(y1, f[x], was.y));
+                } else {
+                  float* at = row + x * JP + d * 16 + quad;
+                  at[0] = fmaf(y0, f[x], round ? at[0] : 0.f);
+                  at[8] = fmaf(y1, f[x], round ? at[8] : 0.f);
+                }
+              }
           }
           __syncthreads();
         }
@@ -715,7 +733,7 @@ extern "C" int d3_paged_attention_workspace_size(int B, int q_heads, int kv_head
              "query heads must be a multiple of key heads");
   D3_REQUIRE(dim == 64 || dim == 128 || dim == 256, "head dim must be 64, 128 or 256");
   const int rows = q_heads / kv_heads > 8 ? 16 : 8;
-  *bytes = static_cast<size_t>(2 * sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
+  *bytes = static_cast<size_t>((dim == 256 ? 2 : 3) * sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
   return D3_OK;
 }
 
@@ -768,12 +786,14 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   a.page_size = cache->page_size;
   a.q_heads = q_heads;
   a.group = q_heads / cache->heads;
-  const bool wide = a.group > 8;  // 16 heads share a read of the keys where there are more than 8
+  // two groups of 8 heads share a read of the keys where there are more than 8
+  const bool wide = a.group > 8;
   a.parts = (a.group + (wide ? 15 : 7)) / (wide ? 16 : 8);
   a.units = cache->heads * a.parts;
   a.scale = scale;
   a.partial = static_cast<float*>(workspace);
-  a.grid = 2 * sm_count();
+  const int D = cache->dim;
+  a.grid = (D == 256 ? 2 : 3) * sm_count();
   a.status = status;
   D3_REQUIRE(aligned(q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0, "rows of q must be 16-byte aligned");
   D3_REQUIRE(aligned(out, 8) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0, "rows of out must be 8-byte aligned");
@@ -782,7 +802,6 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
                  static_cast<int64_t>(B) * q_heads <= 0x7fffffff,
              "batch, heads and length are too large for one call");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int D = cache->dim;
   switch (cache->dtype) {
     case D3_DTYPE_BF16: return wide ? launch_dim<D3_DTYPE_BF16, true>(a, D, s) : launch_dim<D3_DTYPE_BF16, false>(a, D, s);
     case D3_DTYPE_F16: return wide ? launch_dim<D3_DTYPE_F16, true>(a, D, s) : launch_dim<D3_DTYPE_F16, false>(a, D, s);
