@@ -231,18 +231,20 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   float* sRk = sB + 2 * kC;
   float* sRq = sRk + kC;
   float* sScan = sRq + kC;
+  int* found = reinterpret_cast<int*>(sScan + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
   const DeltaArgs& d = a.d;
   const int hk = blockIdx.y;
   pdl_wait();
   pdl_trigger();
-  // the sequence of this record: the last one whose first record is not behind it
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first_record(max(0, __ldg(a.cu + mid)), mid) <= blockIdx.x) lo = mid;
-    else hi = mid - 1;
-  }
+  // the sequence of this record, each thread looking at its own ones
+  if (tid == 0) *found = -1;
+  __syncthreads();
+  for (int i = tid; i < a.n; i += kPrepThreads)
+    if (first_record(max(0, __ldg(a.cu + i)), i) <= blockIdx.x && first_record(max(0, __ldg(a.cu + i + 1)), i + 1) > blockIdx.x) *found = i;
+  __syncthreads();
+  const int lo = *found;
+  if (lo < 0) return;
   const int c0 = max(0, __ldg(a.cu + lo)), c1 = min(a.T, __ldg(a.cu + lo + 1));
   const int64_t chunk = static_cast<int64_t>(blockIdx.x) - first_record(c0, lo);
   if (chunk < 0 || c0 + chunk * kC >= c1) return;

@@ -7,6 +7,10 @@ Drop-in operators with the reference runtime's Python signatures:
   d3moe.experimental_fp8 register, linear (weight-only FP8 dense GEMV)
   d3moe.model            MoEBlock / moe / moe_parts / routed_moe
   d3moe.ep               expert-parallel layer over torch.distributed
+and the sequence memory between the projections of a hybrid decoder:
+  d3moe.attention        kv_append, paged_attention (one new token per sequence)
+  d3moe.gated_delta      gated_delta_step, gated_delta_chunk
+  d3moe.cache            copy_pages, PagedCache
 All compute runs in libd3moe.so (hand-written CUDA for sm_100a) through the C
 ABI of include/d3moe.h; there is no CPU or library fallback.
 """

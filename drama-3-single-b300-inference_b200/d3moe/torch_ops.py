@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import attention, cache, gated_delta, ops
 
 FP8 = torch.float8_e4m3fn
 _ORDERS = ("gate_up", "up_gate")
@@ -111,3 +111,70 @@ def combine_experts_add_norm(routed: torch.Tensor, shared: torch.Tensor, gate: t
 @combine_experts_add_norm.register_fake
 def _(routed, shared, gate, residual, weight, epsilon):
     return residual.new_empty(residual.shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("d3moe::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    seq_lens: torch.Tensor, scale: float | None = None, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, window: int = 0,
+                    max_seq_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse) of d3moe.attention.paged_attention."""
+    return attention.paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale=k_scale,
+                                     v_scale=v_scale, window=window, max_seq_len=max_seq_len, return_lse=True)
+
+
+@paged_attention.register_fake
+def _(q, k_cache, v_cache, page_table, seq_lens, scale=None, k_scale=None, v_scale=None, window=0, max_seq_len=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.custom_op("d3moe::kv_append", mutates_args=("k_cache", "v_cache"))
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              page_table: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None = None,
+              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
+    """d3moe.attention.kv_append; the caches are declared as mutated."""
+    attention.kv_append(k, v, k_cache, v_cache, page_table, positions, seq_ids, k_scale=k_scale, v_scale=v_scale)
+
+
+@kv_append.register_fake
+def _(k, v, k_cache, v_cache, page_table, positions, seq_ids=None, k_scale=None, v_scale=None):
+    return None
+
+
+@torch.library.custom_op("d3moe::copy_pages", mutates_args=("pool",))
+def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0) -> None:
+    """d3moe.cache.copy_pages; the pool is declared as mutated."""
+    cache.copy_pages(pool, src, dst, page_dim)
+
+
+@copy_pages.register_fake
+def _(pool, src, dst, page_dim=0):
+    return None
+
+
+@torch.library.custom_op("d3moe::gated_delta_step", mutates_args=("state",))
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                     state: torch.Tensor, slots: torch.Tensor | None = None, scale: float | None = None,
+                     l2norm: bool = True, eps: float = 1e-6) -> torch.Tensor:
+    """d3moe.gated_delta.gated_delta_step; the state is declared as mutated."""
+    return gated_delta.gated_delta_step(q, k, v, g, beta, state, slots, scale=scale, l2norm=l2norm, eps=eps)
+
+
+@gated_delta_step.register_fake
+def _(q, k, v, g, beta, state, slots=None, scale=None, l2norm=True, eps=1e-6):
+    return v.new_empty(v.shape)
+
+
+@torch.library.custom_op("d3moe::gated_delta_chunk", mutates_args=("state",))
+def gated_delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                      state: torch.Tensor, cu_seqlens: torch.Tensor, slots: torch.Tensor | None = None,
+                      fresh: torch.Tensor | None = None, scale: float | None = None, l2norm: bool = True,
+                      eps: float = 1e-6) -> torch.Tensor:
+    """d3moe.gated_delta.gated_delta_chunk; the state is declared as mutated."""
+    return gated_delta.gated_delta_chunk(q, k, v, g, beta, state, cu_seqlens, slots, fresh=fresh, scale=scale,
+                                         l2norm=l2norm, eps=eps)
+
+
+@gated_delta_chunk.register_fake
+def _(q, k, v, g, beta, state, cu_seqlens, slots=None, fresh=None, scale=None, l2norm=True, eps=1e-6):
+    return v.new_empty(v.shape)
