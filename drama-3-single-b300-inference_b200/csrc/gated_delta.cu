@@ -214,8 +214,66 @@ struct PrepShape {
   static constexpr int kMat = kC * kLd * 4;
   static constexpr int kT = 2 * kMat + 2 * 32 * 20 * 4;  // two heads' T and 16 x 16 products, over the dead tiles
   static constexpr int kTiles = 2 * kTile > kT ? 2 * kTile : kT;
-  static constexpr int kSmem = kTiles + 2 * kMat + (2 * kC * 2 + 2 * kC + 8) * 4;
+  static constexpr int kSmem = kTiles + 2 * kMat + (2 * 4 * kC + 2 * kC * 2 + 2 * kC + 8) * 4;
 };
+
+// exp(G_i - G_j) and the norms times the products of 16-row block I with the keys: P (ROLE
+// 1), or I + A's strictly lower part and B_10 (ROLE 0). Left of the diagonal block the
+// exponential is one factor of the row's by one of the column's, both at most 1.
+template <int ROLE, int I>
+__device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int heads, uint8_t* rec0, const float* sG,
+                                              const float* sB, const float* sRk, const float* sRow, const float* sW,
+                                              float* A, int quad, int t4) {
+  const int i0 = 16 * I + quad;
+#pragma unroll 1
+  for (int h = 0; h < heads; ++h) {
+    const float *hG = sG + h * kC, *hW = sW + (h * 4 + I) * kC + 2 * t4;
+    uint8_t* to = rec0 + h * kRecBytes + (ROLE ? 2 * kRecT : 0) + (i0 * kC + 2 * t4) * 2;
+    float* Ah = A + (h * kC + i0) * kLd + 2 * t4;
+    float g[2], f[2], a[2], b[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      g[half] = hG[i0 + 8 * half];
+      f[half] = sRow[i0 + 8 * half];
+      a[half] = I > 0 ? exp2_fast(g[half] - hG[I > 0 ? 16 * I - 1 : 0]) * f[half] : 0.f;
+      b[half] = ROLE ? 1.f : sB[h * kC + i0 + 8 * half];
+    }
+#pragma unroll
+    for (int n = 0; n < 2 * I + 2; ++n) {
+      const int j = n * 8 + 2 * t4;
+      float e[2][2];
+      if (n < 2 * I) {
+        const float2 w = *reinterpret_cast<const float2*>(hW + n * 8);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          e[half][0] = acc[n][2 * half] * a[half] * w.x;
+          e[half][1] = acc[n][2 * half + 1] * a[half] * w.y;
+        }
+      } else {  // nothing above the diagonal (there the difference may overflow)
+        const float2 gj = *reinterpret_cast<const float2*>(hG + j), rj = *reinterpret_cast<const float2*>(sRk + j);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int i = i0 + 8 * half;
+          e[half][0] = j <= i - (ROLE ? 0 : 1) ? exp2_fast(g[half] - gj.x) * (rj.x * f[half]) * acc[n][2 * half] : 0.f;
+          e[half][1] = j + 1 <= i - (ROLE ? 0 : 1) ? exp2_fast(g[half] - gj.y) * (rj.y * f[half]) * acc[n][2 * half + 1] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (ROLE) {
+          *reinterpret_cast<uint32_t*>(to + half * (8 * kC * 2) + n * 16) = pack16<true>(e[half][0], e[half][1]);
+        } else if (I >= 2 && n < 4) {
+          uint32_t x, y;
+          split_bf16x2(e[half][0], e[half][1], x, y);
+          *reinterpret_cast<uint32_t*>(to + half * (8 * kC * 2) + n * 16) = x;
+          *reinterpret_cast<uint32_t*>(to + kRecT + half * (8 * kC * 2) + n * 16) = y;
+        } else {
+          *reinterpret_cast<float2*>(Ah + half * 8 * kLd + (n & 3) * 8) = make_float2(e[half][0] * b[half], e[half][1] * b[half]);
+        }
+      }
+    }
+  }
+}
 
 // One CTA per (record, key head), two of its value heads at a time. Warps 0-3 make
 // k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads share them.
@@ -226,7 +284,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   float* Tm = reinterpret_cast<float*>(smem);                    // [2][64][kLd]
   float* X = Tm + 2 * kC * kLd;                                  // [2][32][20]
   float* A = reinterpret_cast<float*>(smem + Sh::kTiles);        // [2][64][kLd]
-  float* sG = A + 2 * kC * kLd;  // [2][64] sums of g, in units of log2
+  float* sW = A + 2 * kC * kLd;  // [2][4][64] exp(G at the end of block I - 1 minus G_j) / |k_j|, j before block I
+  float* sG = sW + 2 * 4 * kC;   // [2][64] sums of g, in units of log2
   float* sB = sG + 2 * kC;       // [2][64]
   float* sRk = sB + 2 * kC;
   float* sRq = sRk + kC;
@@ -334,37 +393,21 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
       f[2 * kC + gt] = exp2_fast(end - G) * sRk[gt];
       if (gt == 0) f[3 * kC] = exp2_fast(end);
     }
-    for (int h = 0; h < heads; ++h) {
-      uint8_t* rec = rec0 + h * kRecBytes;
-      const float *hG = sG + h * kC, *hB = sB + h * kC;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int i = rows + quad + 8 * half;
-        const float gi = hG[i], fi = role ? sRq[i] : sRk[i], bi = hB[i];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          if (n * 8 > rows + 8) break;
-          const int j = n * 8 + 2 * t4;
-          const float2 gj = *reinterpret_cast<const float2*>(hG + j), rj = *reinterpret_cast<const float2*>(sRk + j);
-          // exp(G_i - G_j) times the two norms
-          float e0 = exp2_fast(gi - gj.x) * (rj.x * fi) * acc[n][2 * half];
-          float e1 = exp2_fast(gi - gj.y) * (rj.y * fi) * acc[n][2 * half + 1];
-          if (n * 8 >= rows) {  // the diagonal block: nothing above (there the difference may overflow)
-            e0 = j <= i ? e0 : 0.f;
-            e1 = j + 1 <= i ? e1 : 0.f;
-          }
-          if (role) {
-            *reinterpret_cast<uint32_t*>(rec + 2 * kRecT + (i * kC + j) * 2) = pack16<true>(e0, e1);
-          } else if (rows >= 32 && n < 4) {
-            uint32_t x, y;
-            split_bf16x2(e0, e1, x, y);
-            *reinterpret_cast<uint32_t*>(rec + (i * kC + j) * 2) = x;
-            *reinterpret_cast<uint32_t*>(rec + kRecT + (i * kC + j) * 2) = y;
-          } else {
-            *reinterpret_cast<float2*>(A + (h * kC + i) * kLd + (j & 31)) = make_float2(j < i ? e0 * bi : 0.f, j + 1 < i ? e1 * bi : 0.f);
-          }
-        }
-      }
+    for (int e = 0; e < 2; ++e) {
+      const int x = e * kPrepThreads + tid, h = x >> 8, block = (x >> 6) & 3, j = x & (kC - 1);
+      if (j < 16 * block) sW[x] = exp2_fast(sG[h * kC + 16 * block - 1] - sG[h * kC + j]) * sRk[j];
+    }
+    __syncthreads();
+    switch (warp) {  // each with its own straight code: shared and predicated it took twice as long
+      case 0: prep_elements<0, 0>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 1: prep_elements<0, 1>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 2: prep_elements<0, 2>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 3: prep_elements<0, 3>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 4: prep_elements<1, 0>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
+      case 5: prep_elements<1, 1>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
+      case 6: prep_elements<1, 2>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
+      default: prep_elements<1, 3>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
     }
     __syncthreads();
     // (I + A)^-1 of the diagonal blocks of 16, one per warp: columns of the two blocks of
