@@ -194,15 +194,21 @@ struct ChunkArgs {
   int T, n;
 };
 
-// Copies rows [t0, t0 + 64) (zeros from t1 on) of BYTES bytes each into a tile.
+// Copies rows [t0, t0 + 64) (zeros from t1 on) of BYTES bytes each into a tile. A
+// thread's rows are THREADS / PIECES apart (a multiple of 8), so its piece of a row and
+// the permutation of the pieces are the same in all of them.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void load_rows(uint32_t tile, const __nv_bfloat16* src, int64_t stride, int t0, int t1) {
-  constexpr int PIECES = BYTES / 16;
+  constexpr int PIECES = BYTES / 16, STEP = THREADS / PIECES;
+  static_assert(STEP % 8 == 0);
+  const int r = threadIdx.x / PIECES, c = threadIdx.x % PIECES;
+  const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (t0 + r) * stride) + c * 16;
+  const uint32_t to = tile + tile_at<BYTES>(r, c);
+  const int64_t step = STEP * stride * 2;
 #pragma unroll
-  for (int i = 0; i < kC * PIECES / THREADS; ++i) {
-    const int e = i * THREADS + threadIdx.x, r = e / PIECES, c = e % PIECES;
-    const bool take = t0 + r < t1;
-    cp_async_16_zfill(tile + tile_at<BYTES>(r, c), reinterpret_cast<const uint8_t*>(src + (take ? t0 + r : t0) * stride) + c * 16, take);
+  for (int i = 0; i < kC / STEP; ++i, row += step) {
+    const bool take = t0 + r + i * STEP < t1;  // past the end nothing is read
+    cp_async_16_zfill(to + i * STEP * BYTES, take ? row : reinterpret_cast<const uint8_t*>(src), take);
   }
 }
 
@@ -566,7 +572,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
 
   int stage = 0;
   for (int t0 = c0; t0 < c1; t0 += kC, stage ^= 1) {
-    cp_async_wait<1>();  // this chunk's tokens; its matrices may be on their way
+    cp_async_wait<0>();
     __syncthreads();     // and every warp is done with the other stage
     if (t0 + kC < c1) load_tokens(stage ^ 1, t0 + kC, rec + rec_step);
     cp_async_commit();
@@ -574,10 +580,6 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
     const float* f = reinterpret_cast<const float*>(smem + stage * Sh::kStage + Sh::kF);
     // S0^T k_j and S0^T q_j of the chunk's tokens
     float r[8][4], o[8][4];
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) r[n][x] = o[n][x] = 0.f;
 #pragma unroll
     for (int c = 0; c < DK / 16; ++c) {
       uint32_t h[4], l[4];
@@ -591,15 +593,18 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
         ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
+          // only the output sees the product with q: one bf16 term (2^-9) of the state
+          if (c == 0) {
+            mma_16816_first<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
+            mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+          } else {
+            mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
+            mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+          }
           mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
-          // only the output sees this product: one bf16 term (2^-9) of the state
-          mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
         }
       }
     }
-    cp_async_wait<1>();
-    __syncthreads();  // this chunk's matrices are here
     // R = v - exp(G) S0^T k; its two terms as A operands over the tokens
     uint32_t rh[4][4] = {}, rl[4][4] = {};
 #pragma unroll
@@ -626,38 +631,39 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
 #pragma unroll
       for (int y = 0; y < 4; ++y) split_bf16x2(x[2 * k + (y >> 1)][2 * (y & 1)], x[2 * k + (y >> 1)][2 * (y & 1) + 1], h[y], l[y]);
     };
-    // (w0, w1) += rows (tokens) n*8 .. + 15 of the matrix, columns 16 k .. + 15, times block k of x
-    auto times = [&](float (&w0)[4], float (&w1)[4], int n, int k) {
+    // (w0, w1) += (first: =) rows (tokens) n*8 .. + 15 of the matrix, columns 16 k .. + 15, times block k of x
+    auto times = [&](float (&w0)[4], float (&w1)[4], int n, int k, bool first) {
       uint32_t b[4], c[4];
       const uint32_t at = tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi);
       ldmatrix_x4(mat + at, b[0], b[1], b[2], b[3]);
       ldmatrix_x4(mat + kRecT + at, c[0], c[1], c[2], c[3]);
-      mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
-      mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
+      if (first) {
+        mma_16816_first<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
+        mma_16816_first<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
+      } else {
+        mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
+        mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
+      }
       mma_16816<true>(w0, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[0], b[1]);
       mma_16816<true>(w1, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2], b[3]);
       mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[0], c[1]);
       mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[2], c[3]);
     };
     float w[8][4];
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) w[n][x] = 0.f;
     // N_0 = T_0 R_0
     split(r, 0, rh[0], rl[0]);
     split(r, 1, rh[1], rl[1]);
-    times(w[0], w[1], 0, 0);
-    times(w[2], w[3], 2, 0);
-    times(w[2], w[3], 2, 1);
+    times(w[0], w[1], 0, 0, true);
+    times(w[2], w[3], 2, 0, true);
+    times(w[2], w[3], 2, 1, false);
     // R_1 - B_10 N_0
     split(w, 0, rh[0], rl[0]);
     split(w, 1, rh[1], rl[1]);
 #pragma unroll
     for (int n = 4; n < 8; n += 2) {
-      float p[2][4] = {};
-      times(p[0], p[1], n, 0);
-      times(p[0], p[1], n, 1);
+      float p[2][4];
+      times(p[0], p[1], n, 0, true);
+      times(p[0], p[1], n, 1, false);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -666,9 +672,9 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
     // N_1 = T_1 (...)
     split(r, 2, rh[2], rl[2]);
     split(r, 3, rh[3], rl[3]);
-    times(w[4], w[5], 4, 2);
-    times(w[6], w[7], 6, 2);
-    times(w[6], w[7], 6, 3);
+    times(w[4], w[5], 4, 2, true);
+    times(w[6], w[7], 6, 2, true);
+    times(w[6], w[7], 6, 3, false);
     split(w, 2, rh[2], rl[2]);
     split(w, 3, rh[3], rl[3]);
     // out += P N
@@ -714,14 +720,15 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
     const float end = f[3 * kC];
 #pragma unroll
     for (int n = 0; n < DK / 8; n += 2) {
-      float p[2][4] = {};
+      float p[2][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t b[4];
         ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + mtop), b[0], b[1], b[2], b[3]);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
+          if (k == 0) mma_16816_first<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
+          else mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
           mma_16816<true>(p[x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2 * x], b[2 * x + 1]);
         }
       }
