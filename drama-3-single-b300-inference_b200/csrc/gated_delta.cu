@@ -32,6 +32,8 @@
 #include "d3_host.h"
 #include "mma_tiles.cuh"
 
+#include <type_traits>
+
 namespace d3 {
 namespace {
 
@@ -591,18 +593,20 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
         const uint32_t at = tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi);
         ldmatrix_x4(base + at, b[0], b[1], b[2], b[3]);
         ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
+        // (a sum's next product comes four later: it takes about 21 cycles, one issues in 8)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          // only the output sees the product with q: one bf16 term (2^-9) of the state
-          if (c == 0) {
-            mma_16816_first<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
-            mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
-          } else {
-            mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
-            mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
-          }
-          mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
+          if (c == 0) mma_16816_first<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
+          else mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
         }
+        // only the output sees the product with q: one bf16 term (2^-9) of the state
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (c == 0) mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+          else mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
       }
     }
     // R = v - exp(G) S0^T k; its two terms as A operands over the tokens
@@ -631,65 +635,65 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
 #pragma unroll
       for (int y = 0; y < 4; ++y) split_bf16x2(x[2 * k + (y >> 1)][2 * (y & 1)], x[2 * k + (y >> 1)][2 * (y & 1) + 1], h[y], l[y]);
     };
-    // (w0, w1) += (first: =) rows (tokens) n*8 .. + 15 of the matrix, columns 16 k .. + 15, times block k of x
-    auto times = [&](float (&w0)[4], float (&w1)[4], int n, int k, bool first) {
-      uint32_t b[4], c[4];
-      const uint32_t at = tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi);
-      ldmatrix_x4(mat + at, b[0], b[1], b[2], b[3]);
-      ldmatrix_x4(mat + kRecT + at, c[0], c[1], c[2], c[3]);
-      if (first) {
-        mma_16816_first<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
-        mma_16816_first<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
-      } else {
-        mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[0], b[1]);
-        mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2], b[3]);
+    // w += (first: =) rows (tokens) 8 n .. of the matrix, 16 for each of PAIRS pairs, columns
+    // 16 k .. + 15, times block k of x; w: the pairs' accumulators one after the other
+    auto times = [&](auto pairs, float (*w)[4], int n, int k, bool first) {
+      constexpr int PAIRS = decltype(pairs)::value;
+      uint32_t b[PAIRS][4], c[PAIRS][4];
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t at = tile_at<128>((n + 2 * i) * 8 + mtop * 8 + mrow, 2 * k + mhi);
+        ldmatrix_x4(mat + at, b[i][0], b[i][1], b[i][2], b[i][3]);
+        ldmatrix_x4(mat + kRecT + at, c[i][0], c[i][1], c[i][2], c[i][3]);
       }
-      mma_16816<true>(w0, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[0], b[1]);
-      mma_16816<true>(w1, rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2], b[3]);
-      mma_16816<true>(w0, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[0], c[1]);
-      mma_16816<true>(w1, rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[2], c[3]);
+#pragma unroll
+      for (int i = 0; i < 2 * PAIRS; ++i) {
+        if (first) mma_16816_first<true>(w[i], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[i / 2][2 * (i & 1)], b[i / 2][2 * (i & 1) + 1]);
+        else mma_16816<true>(w[i], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[i / 2][2 * (i & 1)], b[i / 2][2 * (i & 1) + 1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * PAIRS; ++i) mma_16816<true>(w[i], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[i / 2][2 * (i & 1)], b[i / 2][2 * (i & 1) + 1]);
+#pragma unroll
+      for (int i = 0; i < 2 * PAIRS; ++i) mma_16816<true>(w[i], rh[k][0], rh[k][1], rh[k][2], rh[k][3], c[i / 2][2 * (i & 1)], c[i / 2][2 * (i & 1) + 1]);
     };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
     float w[8][4];
     // N_0 = T_0 R_0
     split(r, 0, rh[0], rl[0]);
     split(r, 1, rh[1], rl[1]);
-    times(w[0], w[1], 0, 0, true);
-    times(w[2], w[3], 2, 0, true);
-    times(w[2], w[3], 2, 1, false);
+    times(two, w, 0, 0, true);
+    times(one, w + 2, 2, 1, false);
     // R_1 - B_10 N_0
     split(w, 0, rh[0], rl[0]);
     split(w, 1, rh[1], rl[1]);
+    {
+      float p[4][4];
+      times(two, p, 4, 0, true);
+      times(two, p, 4, 1, false);
 #pragma unroll
-    for (int n = 4; n < 8; n += 2) {
-      float p[2][4];
-      times(p[0], p[1], n, 0, true);
-      times(p[0], p[1], n, 1, false);
+      for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 4; ++y) r[n + x][y] -= p[x][y];
+        for (int y = 0; y < 4; ++y) r[4 + x][y] -= p[x][y];
     }
     // N_1 = T_1 (...)
     split(r, 2, rh[2], rl[2]);
     split(r, 3, rh[3], rl[3]);
-    times(w[4], w[5], 4, 2, true);
-    times(w[6], w[7], 6, 2, true);
-    times(w[6], w[7], 6, 3, false);
+    times(two, w + 4, 4, 2, true);
+    times(one, w + 6, 6, 3, false);
     split(w, 2, rh[2], rl[2]);
     split(w, 3, rh[3], rl[3]);
     // out += P N
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      uint32_t b[8][2];
 #pragma unroll
-      for (int n = 2 * k; n < 8; n += 2) {
-        uint32_t b[4];
-        ldmatrix_x4(mat + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[0], b[1], b[2], b[3]);
+      for (int n = 2 * k; n < 8; n += 2)
+        ldmatrix_x4(mat + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[n][0], b[n][1], b[n + 1][0], b[n + 1][1]);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          mma_16816<true>(o[n + x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
-          mma_16816<true>(o[n + x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2 * x], b[2 * x + 1]);
-        }
-      }
+      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[n][0], b[n][1]);
+#pragma unroll
+      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[n][0], b[n][1]);
     }
     __syncthreads();  // every warp is done with the matrices
     rec += rec_step;
@@ -719,21 +723,24 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
       }
     const float end = f[3 * kC];
 #pragma unroll
-    for (int n = 0; n < DK / 8; n += 2) {
-      float p[2][4];
+    for (int n = 0; n < DK / 8; n += 4) {
+      float p[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + mtop), b[0], b[1], b[2], b[3]);
+        uint32_t b[4][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (k == 0) mma_16816_first<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
-          else mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[2 * x], b[2 * x + 1]);
-          mma_16816<true>(p[x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[2 * x], b[2 * x + 1]);
+        for (int x = 0; x < 4; x += 2)
+          ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + x + mtop), b[x][0], b[x][1], b[x + 1][0], b[x + 1][1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (k == 0) mma_16816_first<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
+          else mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
         }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) mma_16816<true>(p[x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[x][0], b[x][1]);
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int y = 0; y < 4; ++y) s[n + x][y] = fmaf(s[n + x][y], end, p[x][y]);
     }
