@@ -58,6 +58,7 @@ struct AttnArgs {
   float scale;
   float* partial;    // [grid][2] records of ROWS * (D + 2) floats
   int grid;          // CTAs of the main kernel
+  int share;         // CTAs of a cluster that shares one unit, 0: the line of all units' tiles
   int32_t* status;
 };
 
@@ -173,6 +174,33 @@ struct Cursor {
   }
 };
 
+// The cluster's CTAs: this one's rank, a barrier over all their threads (what each wrote
+// to its shared memory before is seen by the others after), and reads of CTA c's shared
+// memory at the place that has address `at` in this one's.
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_map(uint32_t at, int c) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(c));
+  return r;
+}
+__device__ __forceinline__ float cluster_load(uint32_t at, int c) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_map(at, c)) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t at, int c) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_map(at, c)) : "memory");
+  return x;
+}
+
 // Four columns of a finished row: x / sum * v_scale in the output's type; lse
 // with the first. A sum of 0 (no key took part) gives zeros and -inf, a NaN stays one.
 template <bool BF16>
@@ -185,7 +213,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int d
     a.lse[static_cast<int64_t>(b) * a.q_heads + h] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * kLn2;
 }
 
-template <int DT, int D, bool WIDE>
+// LINE: a share of the line of all units' tiles; else a cluster per unit.
+template <int DT, int D, bool WIDE, bool LINE>
 __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas)) paged_attention_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool BF16 = DT == D3_DTYPE_BF16;        // type of the matrix products
@@ -205,35 +234,47 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   pdl_wait();
   pdl_trigger();  // after the wait: the joining kernel may read lens before it waits itself
 
-  // where this CTA's share of the line begins
-  const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
-  int mine, before, total;
-  line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
-  const int share = cta_share(total, a.grid);
-  if (total == 0 || static_cast<int64_t>(blockIdx.x) * share >= total) return;
-  const int first = blockIdx.x * share, end = min(first + share, total);
-  if (first >= before && first < before + mine) {
-    int at = before;
-    for (int i = 0; i < per; ++i) {
-      const int b = tid * per + i, n = seq_places<Sh::kTile>(a, b);
-      if (first < at + n) {
-        const int each = n / a.units, unit = (first - at) / each;
-        start[0] = b;
-        start[1] = unit;
-        start[2] = max(0, first - at - unit * each - kUnitCost);
-        start[3] = at + unit * each + kUnitCost + start[2];
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
   Cursor<Sh::kTile> cur;
-  cur.b = start[0];
-  cur.unit = start[1];
-  cur.tile = start[2];
-  cur.at = start[3];
-  if (cur.at >= end) return;  // nothing but a unit's own places
+  int end;  // of this CTA's places
+  const int rank = !LINE && a.share > 1 ? cluster_rank() : 0;
+  if constexpr (!LINE) {  // one unit per cluster, its tiles spread over the CTAs
+    const int id = blockIdx.x / a.share;
+    cur.b = id / a.units;
+    cur.unit = id % a.units;
+    const int tiles = seq_tiles<Sh::kTile>(a, cur.b);
+    cur.tile = cur.at = rank * tiles / a.share;
+    end = (rank + 1) * tiles / a.share;
+  } else {
+    // where this CTA's share of the line begins
+    const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
+    int mine, before, total;
+    line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
+    const int share = cta_share(total, a.grid);
+    if (total == 0 || static_cast<int64_t>(blockIdx.x) * share >= total) return;
+    const int first = blockIdx.x * share;
+    end = min(first + share, total);
+    if (first >= before && first < before + mine) {
+      int at = before;
+      for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i, n = seq_places<Sh::kTile>(a, b);
+        if (first < at + n) {
+          const int each = n / a.units, unit = (first - at) / each;
+          start[0] = b;
+          start[1] = unit;
+          start[2] = max(0, first - at - unit * each - kUnitCost);
+          start[3] = at + unit * each + kUnitCost + start[2];
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+    cur.b = start[0];
+    cur.unit = start[1];
+    cur.tile = start[2];
+    cur.at = start[3];
+    if (cur.at >= end) return;  // nothing but a unit's own places
+  }
   cur.enter(a);
   Cursor<Sh::kTile> ld = cur;
 
@@ -304,7 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   };
 
   fetch_q(cur);
-  look_up();
+  if (ld.at < end) look_up();
 #pragma unroll
   for (int s = 0; s < P; ++s) {
     load_keys();
@@ -319,8 +360,11 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   float m[NH][2], l[NH][2];  // of heads 2 t4 and 2 t4 + 1
   float lg[NH][2];         // their logits in units of log2, per product
   bool opened = false, whole = false;
+  float* shared_rec = reinterpret_cast<float*>(smem);
+  const int unit0 = cur.unit, b0 = cur.b;
+  const bool empty = cur.at >= end;
   int seg_slot = 0, use = 0;
-  bool more = true;
+  bool more = cur.at < end;
   for (bool begun = false; more; begun = true) {
     const int head = cur.unit / a.parts;
     const int h0 = head * a.group + (cur.unit % a.parts) * ROWS;
@@ -533,8 +577,13 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
           }
         }
       __syncthreads();
-      whole = whole && last;
+      whole = whole && last && (LINE || a.share < 2);
       float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
+      if (!LINE && a.share > 1) {  // for the cluster: over the ring, which nothing is on its way to any more
+        cp_async_wait<0>();
+        __syncthreads();
+        rec = shared_rec;
+      }
       const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
       // each warp scales its rows to the common maximum; JW at a time they are
       // added into JW buffers, in the order of the warps
@@ -606,6 +655,41 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
     cur = nxt;
   }
   cp_async_wait<0>();
+  if (LINE || (a.share == 1 && !empty)) return;
+
+  // join the cluster: CTA r takes the rows r, r + share, ... of all its CTAs' records
+  // (one CTA alone comes here for a sequence without keys)
+  if (empty)
+    for (int r = tid; r < ROWS; r += kAttnThreads) {
+      shared_rec[ROWS * D + r] = -INFINITY;
+      shared_rec[ROWS * D + ROWS + r] = 0.f;
+    }
+  if (a.share > 1) cluster_sync();
+  else __syncthreads();
+  const int head = unit0 / a.parts, h0 = head * a.group + (unit0 % a.parts) * ROWS;
+  const int nh = min(ROWS, (head + 1) * a.group - h0);
+  const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
+  const uint32_t rec = smem_u32(smem);
+  for (int e = tid * 4; e < ((nh - rank + a.share - 1) / a.share) * D; e += kAttnThreads * 4) {
+    const int r = rank + e / D * a.share, d = e % D;
+    float top = -INFINITY, sum = 0.f, x[4] = {};
+    for (int c = 0; c < a.share; ++c) top = fmaxf(top, cluster_load(rec + (ROWS * D + r) * 4, c));
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+    for (int c = 0; c < a.share; ++c) {
+      const float m = cluster_load(rec + (ROWS * D + r) * 4, c), l = cluster_load(rec + (ROWS * D + ROWS + r) * 4, c);
+      if (m == -INFINITY && l == 0.f) continue;  // no key: its row was never written
+      const float f = exp2f(m - base);
+      const float4 y = cluster_load4(rec + (r * D + d) * 4, c);
+      sum = fmaf(f, l, sum);
+      x[0] = fmaf(f, y.x, x[0]);
+      x[1] = fmaf(f, y.y, x[1]);
+      x[2] = fmaf(f, y.z, x[2]);
+      x[3] = fmaf(f, y.w, x[3]);
+    }
+    store_row<QBF16>(a, b0, h0 + r, d, x, sum, top, vsc);
+  }
+  if (a.share > 1) cluster_sync();  // no CTA's shared memory goes away while another reads it
 }
 
 // One CTA per query row: rows without keys get zeros, rows of units that several
@@ -698,6 +782,18 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   store_row<QBF16>(a, b, h, d * 4, out, sum, top, a.v_scale ? __ldg(a.v_scale + head) : 1.0f);
 }
 
+// How units of up to `tiles` tiles each are taken: by clusters of the returned number of
+// CTAs (1: whole), or 0: all units' tiles as one line. Measured on 64-tile steps (bf16, 2
+// key heads of 256, us whole / cluster / line): 1 sequence of 256 tokens 10.6 / 8.3 / 9.1,
+// of 1024 27.9 / 10.4 / 10.8; 64 sequences of up to 256 11.4 / 11.9 / 13.4, of up to 1024
+// 30.7 / - / 23.6.
+int unit_ctas(int tiles, int64_t units, int grid) {
+  if (tiles <= 2 || (tiles <= 6 && units * 4 >= grid)) return 1;  // short, or enough of them to fill the GPU
+  int n = 8;
+  while (n > 1 && (n / 2 >= tiles || units * n > grid)) n /= 2;
+  return n > 1 && (tiles + n - 1) / n <= 3 ? n : 0;
+}
+
 template <int DT, int D, bool WIDE>
 int launch_attention(AttnArgs& a, cudaStream_t s) {
   using Sh = AttnShape<DT, D, WIDE>;
@@ -705,11 +801,31 @@ int launch_attention(AttnArgs& a, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    if (cudaFuncSetAttribute(paged_attention_kernel<DT, D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(paged_attention_kernel<DT, D, WIDE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(paged_attention_kernel<DT, D, WIDE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem) != cudaSuccess)
       return check_launch("d3_paged_attention");
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  launch_kernel(paged_attention_kernel<DT, D, WIDE>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
+  const int keys = a.window > 0 && a.window < a.max_len ? a.window : a.max_len;
+  a.share = unit_ctas((keys + Sh::kTile - 1) / Sh::kTile, static_cast<int64_t>(a.B) * a.units, a.grid);
+  if (a.share > 0) {  // one launch: units of their own, or clusters that join by themselves
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.B * a.units * a.share));
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = Sh::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(a.share);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.share > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, paged_attention_kernel<DT, D, WIDE, false>, static_cast<AttnArgs>(a));
+    return check_launch("d3_paged_attention");
+  }
+  launch_kernel(paged_attention_kernel<DT, D, WIDE, true>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
   launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.q_heads)), dim3(kAttnThreads),
                 kAttnThreads * 16 + (a.grid + 3 * kAttnWarps + 1) * 4, s, a);
   return check_launch("d3_paged_attention");
