@@ -62,20 +62,25 @@ struct AttnArgs {
   int32_t* status;
 };
 
+constexpr int attn_ctas(int D, int elem) { return D * elem >= 256 ? 2 : 3; }
+
 // Sizes of one variant. WIDE: 16 query heads per unit, else 8.
 template <int DT, int D, bool WIDE>
 struct AttnShape {
   static constexpr int kElem = DT == D3_DTYPE_E4M3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  // CTAs that share an SM, and what of its shared memory one may take
-  static constexpr int kCtas = D == 256 ? 2 : 3;
-  static constexpr int kMaxSmem = (D == 256 ? 113 : 75) * 1024;
+  // CTAs that share an SM, and what of its shared memory one may take: two with deep rings
+  // for rows of 256 bytes and more, three for shorter ones, which need more work per byte (16
+  // sequences of up to 8000 tokens, 8 bf16 key heads of 128: 60 us with two, 75 with
+  // three; of up to 16000, e4m3: 65 and 64, of 64 columns 52 and 47)
+  static constexpr int kCtas = attn_ctas(D, kElem);
+  static constexpr int kMaxSmem = (kCtas == 2 ? 113 : 75) * 1024;
   // keys of one warp and tile, 16 or 32: a slot of the ring holds 8 KB for 256 columns, up to 4 KB else
   static constexpr int kNK = kRowBytes == 256 || kRowBytes == 512 ? (D == 256 && kElem == 1 ? 32 : 16) : 32;
   static constexpr int kTile = kNK * kAttnWarps;
   static constexpr int kRows = WIDE ? 16 : 8;
   static constexpr int kHalf = kNK * kRowBytes;  // bytes of a slot
-  static constexpr int kFit = ((D == 256 ? 24576 : 16384) / kHalf - 1) / 2;
+  static constexpr int kFit = ((kCtas == 2 ? 24576 : 16384) / kHalf - 1) / 2;
   static constexpr int kAhead = kFit < 4 ? kFit : 4;  // tiles loaded ahead
   static constexpr int kSlots = 2 * kAhead + 1;
   static constexpr int kWarpRing = kSlots * kHalf;
@@ -849,7 +854,7 @@ extern "C" int d3_paged_attention_workspace_size(int B, int q_heads, int kv_head
              "query heads must be a multiple of key heads");
   D3_REQUIRE(dim == 64 || dim == 128 || dim == 256, "head dim must be 64, 128 or 256");
   const int rows = q_heads / kv_heads > 8 ? 16 : 8;
-  *bytes = static_cast<size_t>((dim == 256 ? 2 : 3) * sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
+  *bytes = static_cast<size_t>(attn_ctas(dim, 1) * sm_count()) * 2 * rows * (dim + 2) * sizeof(float);
   return D3_OK;
 }
 
@@ -909,7 +914,7 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   a.scale = scale;
   a.partial = static_cast<float*>(workspace);
   const int D = cache->dim;
-  a.grid = (D == 256 ? 2 : 3) * sm_count();
+  a.grid = attn_ctas(D, static_cast<int>(e)) * sm_count();
   a.status = status;
   D3_REQUIRE(aligned(q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0, "rows of q must be 16-byte aligned");
   D3_REQUIRE(aligned(out, 8) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0, "rows of out must be 8-byte aligned");
