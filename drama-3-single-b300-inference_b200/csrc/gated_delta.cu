@@ -9,7 +9,9 @@
 // One CTA per (sequence, value head, 32 value columns): thread (row group,
 // column quad) keeps consecutive rows of 4 columns in registers. Everything a CTA
 // reads is asked for at once, and the sums over the rows (with those of q.q, k.k and
-// k.q, which give the norms) meet in one exchange.
+// k.q, which give the norms) meet in one exchange. Bound by HBM: 64 sequences of 32
+// heads of 128 x 128 (268 MB of state in and out) take 43.5 us, 6.2 TB/s or 0.96 of the
+// copy rate; with the gates and values asked for after the exchange it was 48.5 us.
 //
 // Packed prompts go in chunks of 64 tokens. With G_i the sum of g up to token i
 // of the chunk, k_i and q_i the normalised keys and scaled queries, and S0 the state
@@ -24,10 +26,24 @@
 //   N_0 = T_0 R_0,   N_1 = T_1 (R_1 - B_10 N_0).
 // A first kernel makes T_0, T_1, B_10 and P for all chunks in parallel (they do not
 // need the state); a second one walks each sequence's chunks with the state in
-// registers. What follows from products of 16-bit factors runs on
-// mma.sync; the state has to stay exact to fp32's neighbourhood, so every factor of
-// a product that reaches it (S0, R, N, T) is split into two bf16 terms (2^-17),
-// and the keys are taken as they come, bf16, with their norms as factors outside.
+// registers.
+//
+// Rounding. All products run on mma.sync with bf16 factors and fp32 sums. Every factor of
+// a product that reaches the state (S0, R, N, T, B) goes in two bf16 terms, 2^-17 of
+// itself (together 2e-6 to 5e-6 of the state's norm after thousands of tokens); keys,
+// queries and values are bf16 as they come, their norms factors outside. What only an
+// output sees (S0 beside the queries, P) goes in one term, 2^-9, like the output itself.
+// Three terms would cost half as many products again.
+//
+// What bounds it. The state passes from chunk to chunk, so a sequence of 2048 tokens is 32
+// steps of 3.4 us however much of the GPU is free (126 us in all, 113 of them the walk);
+// of a step's 6500 cycles per warp 3360 are tensor (420 products of 8), the rest the
+// splitting, the short dependent products of the solve, and loads and stores. 64
+// ragged prompts of 32 heads (17.5k tokens) take 552 us: the walk 425 at 0.59 of the
+// rate of mma.sync and 0.25 of HBM's, the first kernel 130. tcgen05 was not taken: the
+// state would go through tensor memory and registers five times a chunk (state, R, N and
+// their terms), 500 columns of 32 lanes and about 2000 instructions a thread, as long as
+// the walk takes now at a few percent of that unit.
 #include "d3_common.cuh"
 #include "d3_host.h"
 #include "mma_tiles.cuh"
@@ -283,7 +299,9 @@ __device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int head
   }
 }
 
-// One CTA per (record, key head), two of its value heads at a time. Warps 0-3 make
+// One CTA per (record, key head), two of its value heads at a time: bound by latency and
+// instructions, not by its 279 MB (138 us for 305 chunks of 16 key heads, 43% of issue
+// slots busy with four CTAs on an SM). Warps 0-3 make
 // k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads share them.
 template <int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const ChunkArgs a) {
@@ -376,7 +394,10 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
     __syncthreads();  // the tiles, or the previous heads' matrices, are no longer read
     float G = 0.f;
     if (tid < 2 * kC) {
+      // (a decay to below 2^-126 is 0 either way; the bound keeps later differences exact
+      // and takes g = -infinity, a reset)
       G = g_next * 1.4426950408889634f;
+      G = G < -150.f ? -150.f : G;
       sB[tid] = b_next;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -522,7 +543,9 @@ struct WalkShape {
 // chunks. Warp w holds the transposed state of its 16 value columns, [16, DK], as
 // mma accumulators: these are laid out like A operands, so the state, R and N go from
 // product to product in registers, and warps share only what they read (keys,
-// queries, T, P), which cp.async brings one chunk ahead.
+// queries, T, P), which cp.async brings one chunk ahead. (A full 64 x 64 inverse in place
+// of the two halves cost the first kernel more than it saved here; 8 warps on 128
+// columns, one CTA per SM, took the same; loads spread between the products too.)
 template <int DK, int DV>
 __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const ChunkArgs a) {
   using Sh = WalkShape<DK>;

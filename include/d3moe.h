@@ -1,5 +1,6 @@
 /*
- * d3moe.h — C ABI of the B200 (sm_100a) FP8 mixture-of-experts hot path.
+ * d3moe.h — C ABI of the B200 (sm_100a) FP8 mixture-of-experts hot path, and of the
+ * sequence memory (paged attention, gated delta rule) between its projections.
  *
  * Every entry point is stream-ordered (it only enqueues work on `stream`),
  * performs no device or pinned allocation and never synchronises the device.
@@ -517,7 +518,7 @@ D3_API int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q_hea
  * where q and k are key head h / (value_heads / key_heads), divided by
  * sqrt(|x|^2 + eps) first when l2norm is not 0. q, k bf16 [T, key_heads,
  * key_dim]; v, out bf16 [T, value_heads, value_dim] (token strides in elements,
- * heads and dims contiguous); g (log decay, <= 0), beta f32 [T, value_heads]
+ * heads and dims contiguous); g (log decay, <= 0; -infinity resets), beta f32 [T, value_heads]
  * (token strides in elements). state f32 [slots, value_heads, key_dim,
  * value_dim] (slot stride in elements) is updated in place. key_dim and
  * value_dim 64 or 128; q, k, v, out rows and the state 16-byte aligned.

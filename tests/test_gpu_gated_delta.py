@@ -122,6 +122,23 @@ def test_chunk_zero_rows_and_zero_beta():
     assert R.rel_l2(state[0], before[0].double() * torch.exp(g.double().sum(0))[:, None, None]) <= STATE_TOL
 
 
+def test_chunk_resets():
+    """A log decay of -infinity (or far below what fp32 holds) forgets everything before its token."""
+    from d3moe import gated_delta
+    q, k, v, g, beta = operands(150, 2, 4, 128, 128, seed=8)
+    g[[20, 63, 64, 100], 1:3] = -math.inf
+    g[[5, 90], 0] = -1e4
+    state = pool(1, 4, 128, 128)
+    before = state.clone()
+    out = gated_delta.gated_delta_chunk(q, k, v, g, beta, state, torch.tensor([0, 150], dtype=torch.int32, device="cuda"))
+    want, ws = R.delta(q, k, v, g, beta, before, [(0, 150)], [0], 128 ** -0.5)
+    assert R.rel_l2(out, want) <= OUT_TOL and R.rel_l2(state, ws) <= STATE_TOL
+    a, b = before.clone(), before.clone()
+    gated_delta.gated_delta_step(q[20:21], k[20:21], v[20:21], g[20:21], beta[20:21], a)
+    _, b = R.delta(q[20:21], k[20:21], v[20:21], g[20:21], beta[20:21], b, [(0, 1)], [0], 128 ** -0.5)
+    assert R.rel_l2(a, b) <= STEP_STATE_TOL
+
+
 def test_chunk_many_sequences_and_determinism():
     lens = [(7 * i) % 90 for i in range(150)]
     a = chunk(lens, (1, 2, 64, 64), seed=5)
