@@ -137,8 +137,8 @@ __device__ __forceinline__ int cta_share(int total, int grid) {
 
 // Sums over the sequences with all threads: the places of all
 // sequences, and each thread's exclusive prefix over its own run of `per`
-// sequences. scratch: kAttnWarps values of shared memory.
-template <int TILE>
+// sequences. scratch: WARPS values of shared memory.
+template <int TILE, int WARPS>
 __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int* scratch, int& mine, int& before,
                                           int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -158,7 +158,7 @@ __device__ __forceinline__ void line_scan(const AttnArgs& a, int per, int* scrat
   before = x - mine;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += scratch[w];
     total += scratch[w];
   }
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
     // where this CTA's share of the line begins
     const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
     int mine, before, total;
-    line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
+    line_scan<Sh::kTile, kAttnWarps>(a, per, scratch, mine, before, total);
     const int share = cta_share(total, a.grid);
     if (total == 0 || static_cast<int64_t>(blockIdx.x) * share >= total) return;
     const int first = blockIdx.x * share;
@@ -706,29 +706,31 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   if (a.share > 1) cluster_sync();  // no CTA's shared memory goes away while another reads it
 }
 
+constexpr int kGatherWarps = 8, kGatherThreads = kGatherWarps * 32;
+
 // One CTA per query row: rows without keys get zeros, rows of units that several
 // CTAs shared are joined from their records. Groups of D / 4 threads add up every
-// (256 * 4 / D)-th record, so the loads of a long unit's records overlap; the
+// (kGatherThreads * 4 / D)-th record, so the loads of a long unit's records overlap; the
 // groups are then added in order.
 template <int DT, int D, bool WIDE>
-__global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool QBF16 = DT != D3_DTYPE_F16;
-  constexpr int ROWS = Sh::kRows, LANES = D / 4, GROUPS = kAttnThreads / LANES;
+  constexpr int ROWS = Sh::kRows, LANES = D / 4, GROUPS = kGatherThreads / LANES;
   extern __shared__ __align__(1024) uint8_t smem[];
   float4* acc = reinterpret_cast<float4*>(smem);                       // [GROUPS][LANES]
-  float* fac = reinterpret_cast<float*>(smem) + kAttnThreads * 4;      // [a.grid] maximum, then weight
+  float* fac = reinterpret_cast<float*>(smem) + kGatherThreads * 4;      // [a.grid] maximum, then weight
   float* red = fac + a.grid;                                           // [2][warps]
-  int* scratch = reinterpret_cast<int*>(red + 2 * kAttnWarps);
-  int* found = scratch + kAttnWarps;
+  int* scratch = reinterpret_cast<int*>(red + 2 * kGatherWarps);
+  int* found = scratch + kGatherWarps;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads;
   const int head = h / a.group, part = (h - head * a.group) / ROWS, r = (h - head * a.group) % ROWS;
   const int unit = head * a.parts + part;
-  const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
+  const int per = (a.B + kGatherThreads - 1) / kGatherThreads;
   pdl_trigger();
   int mine, before, total;
-  line_scan<Sh::kTile>(a, per, scratch, mine, before, total);
+  line_scan<Sh::kTile, kGatherWarps>(a, per, scratch, mine, before, total);
   const int tiles = seq_tiles<Sh::kTile>(a, b);
   if (b / per == tid) {
     int at = before;
@@ -748,7 +750,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   const float* rec = a.partial + static_cast<int64_t>(c0) * 2 * Sh::kRecord;  // + 2 c records, c > 0
   auto record = [&](int c) { return c == 0 ? rec0 : rec + static_cast<int64_t>(c) * 2 * Sh::kRecord; };
   float top = -INFINITY, sum = 0.f;
-  for (int c = tid; c < n; c += kAttnThreads) {
+  for (int c = tid; c < n; c += kGatherThreads) {
     const float m = __ldcg(record(c) + ROWS * D + r);
     fac[c] = m;
     top = fmaxf(top, m);
@@ -757,16 +759,16 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   if (lane == 0) red[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, red[w]);
+  for (int w = 0; w < kGatherWarps; ++w) top = fmaxf(top, red[w]);
   const float base = top == -INFINITY ? 0.f : top;
-  for (int c = tid; c < n; c += kAttnThreads) {
+  for (int c = tid; c < n; c += kGatherThreads) {
     const float f = exp2f(fac[c] - base);
     fac[c] = f;
     sum += f * __ldcg(record(c) + ROWS * D + ROWS + r);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red[kAttnWarps + warp] = sum;
+  if (lane == 0) red[kGatherWarps + warp] = sum;
   __syncthreads();
   const int d = tid % LANES, g = tid / LANES;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(kAttnThreads) paged_attention_join_kernel(cons
   float out[4] = {};
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kAttnWarps; ++w) sum += red[kAttnWarps + w];
+  for (int w = 0; w < kGatherWarps; ++w) sum += red[kGatherWarps + w];
   for (int i = 0; i < GROUPS; ++i) {
     const float4 y = acc[i * LANES + d];
     out[0] += y.x;
@@ -840,8 +842,8 @@ int launch_attention(AttnArgs& a, cudaStream_t s) {
     return check_launch("d3_paged_attention");
   }
   launch_kernel(paged_attention_kernel<DT, D, WIDE, true>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
-  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.q_heads)), dim3(kAttnThreads),
-                kAttnThreads * 16 + (a.grid + 3 * kAttnWarps + 1) * 4, s, a);
+  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.q_heads)), dim3(kGatherThreads),
+                kGatherThreads * 16 + (a.grid + 3 * kGatherWarps + 1) * 4, s, a);
   return check_launch("d3_paged_attention");
 }
 
