@@ -216,10 +216,10 @@ struct ChunkArgs {
 // thread's rows are THREADS / PIECES apart (a multiple of 8), so its piece of a row and
 // the permutation of the pieces are the same in all of them.
 template <int BYTES, int THREADS>
-__device__ __forceinline__ void load_rows(uint32_t tile, const __nv_bfloat16* src, int64_t stride, int t0, int t1) {
+__device__ __forceinline__ void load_rows(uint32_t tile, const __nv_bfloat16* src, int64_t stride, int t0, int t1, int thread) {
   constexpr int PIECES = BYTES / 16, STEP = THREADS / PIECES;
   static_assert(STEP % 8 == 0);
-  const int r = threadIdx.x / PIECES, c = threadIdx.x % PIECES;
+  const int r = thread / PIECES, c = thread % PIECES;
   const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (t0 + r) * stride) + c * 16;
   const uint32_t to = tile + tile_at<BYTES>(r, c);
   const int64_t step = STEP * stride * 2;
@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   const int t0 = c0 + static_cast<int>(chunk) * kC, nt = min(kC, c1 - t0);
 
   const uint32_t kt = smem_u32(smem), qt = kt + Sh::kTile;
-  load_rows<DK * 2, kPrepThreads>(kt, d.k + hk * DK, d.k_stride, t0, c1);
-  load_rows<DK * 2, kPrepThreads>(qt, d.q + hk * DK, d.q_stride, t0, c1);
+  load_rows<DK * 2, kPrepThreads>(kt, d.k + hk * DK, d.k_stride, t0, c1, tid);
+  load_rows<DK * 2, kPrepThreads>(qt, d.q + hk * DK, d.q_stride, t0, c1, tid);
   cp_async_commit();
   // decays and step sizes of the first two heads, on their way meanwhile
   const int gh = tid >> 6, gt = tid & (kC - 1);  // (threads 0-127) head, token
@@ -528,15 +528,18 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
 
 constexpr int kWalkWarps = 4, kWalkThreads = kWalkWarps * 32, kWalkCols = 16 * kWalkWarps;
 
-// Two CTAs share an SM: keys, queries, values and factors of two chunks, and T and P of
-// one, whose place is free again by the time the state is updated.
-template <int DK>
+// Shared memory: keys, queries, values and factors of two chunks, and T and P of one, whose
+// place is free again by the time the state is updated, so that two CTAs share an SM. With
+// PAIR (below) T and P of two, and what the warps of a pair hand over.
+template <int DK, bool PAIR>
 struct WalkShape {
   static constexpr int kKT = kC * DK * 2, kV = kC * kWalkCols * 2;
-  static constexpr int kQ = kKT, kVAt = 2 * kKT, kF = kVAt + kV, kStage = kF + 1024;
-  static constexpr int kRec = 2 * kStage;
-  static constexpr int kSmem = kRec + 3 * kRecT;
-  static_assert(kSmem <= 113 * 1024);
+  static constexpr int kQ = kKT, kVAt = 2 * kKT, kF = kVAt + kV, kMat = kF + 1024;
+  static constexpr int kStage = kMat + (PAIR ? 3 * kRecT : 0);
+  static constexpr int kRec = 2 * kStage;  // the matrices, or the pairs' places
+  static constexpr int kPairS = DK / 16 * 512, kPair = kPairS + 8 * 512;
+  static constexpr int kSmem = kRec + (PAIR ? kWalkWarps * kPair : 3 * kRecT);
+  static_assert(kSmem <= (PAIR ? 227 : 113) * 1024);
 };
 
 // One CTA per (64 value columns, value head, sequence) walks the sequence's
@@ -546,12 +549,22 @@ struct WalkShape {
 // queries, T, P), which cp.async brings one chunk ahead. (A full 64 x 64 inverse in place
 // of the two halves cost the first kernel more than it saved here; 8 warps on 128
 // columns, one CTA per SM, took the same; loads spread between the products too.)
-template <int DK, int DV>
-__global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const ChunkArgs a) {
-  using Sh = WalkShape<DK>;
-  constexpr int VR = kWalkCols * 2;
+//
+// PAIR, for few CTAs, where a chunk's latency is what counts: each warp has a second one
+// beside it that takes what the next chunk does not wait for, the loads, S0^T q, P N and the
+// output. It gets the state's first terms and N as the A operands they are, through
+// shared memory (two named barriers a chunk). 2048 tokens of one sequence: 126 us without,
+// 106 with. With many CTAs it would only take the place of a second CTA's warps.
+template <int DK, int DV, bool PAIR>
+__global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_delta_walk_kernel(const ChunkArgs a) {
+  using Sh = WalkShape<DK, PAIR>;
+  constexpr int VR = kWalkCols * 2, THREADS = kWalkThreads * (PAIR ? 2 : 1);
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
+  const int warp = (tid >> 5) & (kWalkWarps - 1);        // its 16 columns
+  const bool second = PAIR && tid >= kWalkThreads;     // the pair's second warp
+  const bool loads = !PAIR || second;
+  const int lt = PAIR ? tid - kWalkThreads : tid;        // number among those that load
   const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
   const DeltaArgs& d = a.d;
   const int seq = blockIdx.z, hv = blockIdx.y, hk = hv / d.rep;
@@ -561,7 +574,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
   const int c0 = max(0, __ldg(a.cu + seq)), c1 = min(a.T, __ldg(a.cu + seq + 1));
   const int slot = delta_slot(d, seq);
   if (slot < 0) {
-    for (int e = tid; e < (c1 - c0) * (kWalkCols / 8); e += kWalkThreads)
+    for (int e = tid; e < (c1 - c0) * (kWalkCols / 8); e += THREADS)
       *reinterpret_cast<uint4*>(d.out + (c0 + e / (kWalkCols / 8)) * d.out_stride + hv * DV + col + e % (kWalkCols / 8) * 8) = make_uint4(0, 0, 0, 0);
     return;
   }
@@ -570,52 +583,123 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
   const uint32_t sm = smem_u32(smem);
   auto load_tokens = [&](int stage, int t0, const uint8_t* rec) {
     const uint32_t s = sm + stage * Sh::kStage;
-    load_rows<DK * 2, kWalkThreads>(s, d.k + hk * DK, d.k_stride, t0, c1);
-    load_rows<DK * 2, kWalkThreads>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1);
-    load_rows<VR, kWalkThreads>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1);
-    if (tid < 49) cp_async_16(smem + stage * Sh::kStage + Sh::kF + tid * 16, rec + kRecScal + tid * 16);
+    load_rows<DK * 2, kWalkThreads>(s, d.k + hk * DK, d.k_stride, t0, c1, lt);
+    load_rows<DK * 2, kWalkThreads>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1, lt);
+    load_rows<VR, kWalkThreads>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1, lt);
+    if (lt < 49) cp_async_16(smem + stage * Sh::kStage + Sh::kF + lt * 16, rec + kRecScal + lt * 16);
   };
-  auto load_matrices = [&](const uint8_t* rec) {  // blocks up to the diagonal
+  auto load_matrices = [&](int stage, const uint8_t* rec) {  // blocks up to the diagonal
+    uint8_t* to = smem + (PAIR ? stage * Sh::kStage + Sh::kMat : Sh::kRec);
 #pragma unroll
     for (int i = 0; i < 3 * kC * 8 / kWalkThreads; ++i) {
-      const int e = i * kWalkThreads + tid, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
-      if (c < (r >> 4) * 2 + 2) cp_async_16(smem + Sh::kRec + m * kRecT + tile_at<128>(r, c), rec + m * kRecT + r * 128 + c * 16);
+      const int e = i * kWalkThreads + lt, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
+      if (c < (r >> 4) * 2 + 2) cp_async_16(to + m * kRecT + tile_at<128>(r, c), rec + m * kRecT + r * 128 + c * 16);
     }
   };
   float* S = d.state + slot * d.slot_stride + static_cast<int64_t>(hv) * DK * DV + col + 16 * warp;
   float s[DK / 8][4];
   const bool zero = a.fresh && a.fresh[seq];
-  if (c0 < c1) load_tokens(0, c0, rec);
-  cp_async_commit();
-  if (c0 < c1) load_matrices(rec);
+  if (loads && c0 < c1) {
+    load_tokens(0, c0, rec);
+    load_matrices(0, rec);
+  }
   cp_async_commit();
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      s[n][x] = zero ? 0.f : S[(n * 8 + 2 * t4 + (x & 1)) * DV + quad + (x >> 1) * 8];
+      s[n][x] = zero || second ? 0.f : S[(n * 8 + 2 * t4 + (x & 1)) * DV + quad + (x >> 1) * 8];
 
   int stage = 0;
   for (int t0 = c0; t0 < c1; t0 += kC, stage ^= 1) {
     cp_async_wait<0>();
     __syncthreads();     // and every warp is done with the other stage
-    if (t0 + kC < c1) load_tokens(stage ^ 1, t0 + kC, rec + rec_step);
+    if (loads && t0 + kC < c1) {
+      load_tokens(stage ^ 1, t0 + kC, rec + rec_step);
+      if (PAIR) load_matrices(stage ^ 1, rec + rec_step);
+    }
     cp_async_commit();
-    const uint32_t base = sm + stage * Sh::kStage, mat = sm + Sh::kRec;
+    const uint32_t base = sm + stage * Sh::kStage, mat = PAIR ? base + Sh::kMat : sm + Sh::kRec;
     const float* f = reinterpret_cast<const float*>(smem + stage * Sh::kStage + Sh::kF);
+    float o[8][4];
+    // out += P N's block k, which has the terms h and l
+    auto add_pn = [&](int k, const uint32_t (&h)[4], const uint32_t (&l)[4]) {
+      uint32_t b[8][2];
+#pragma unroll
+      for (int n = 2 * k; n < 8; n += 2)
+        ldmatrix_x4(mat + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[n][0], b[n][1], b[n + 1][0], b[n + 1][1]);
+#pragma unroll
+      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], h[0], h[1], h[2], h[3], b[n][0], b[n][1]);
+#pragma unroll
+      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], l[0], l[1], l[2], l[3], b[n][0], b[n][1]);
+    };
+    // the output's 16 columns of 64 tokens, turned in shared memory: in the place of the
+    // values, which no other pair reads
+    auto put_out = [&]() {
+#pragma unroll
+      for (int n = 0; n < 8; n += 2)
+        stmatrix_x4_trans(base + Sh::kVAt + tile_at<VR>(n * 8 + mtop * 8 + mrow, 2 * warp + mhi), pack16<true>(o[n][0], o[n][1]),
+                          pack16<true>(o[n][2], o[n][3]), pack16<true>(o[n + 1][0], o[n + 1][1]), pack16<true>(o[n + 1][2], o[n + 1][3]));
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = i * 16 + (lane >> 1);
+        if (t0 + t < c1)
+          *reinterpret_cast<uint4*>(d.out + (t0 + t) * d.out_stride + hv * DV + col + 16 * warp + (lane & 1) * 8) =
+              *reinterpret_cast<const uint4*>(smem + stage * Sh::kStage + Sh::kVAt + tile_at<VR>(t, 2 * warp + (lane & 1)));
+      }
+    };
+    auto scale_out = [&](int n) {  // by exp(G) scale / |q|
+      const float2 g = *reinterpret_cast<const float2*>(f + kC + n * 8 + 2 * t4);
+      o[n][0] *= g.x;
+      o[n][1] *= g.y;
+      o[n][2] *= g.x;
+      o[n][3] *= g.y;
+    };
+    uint4* pair = reinterpret_cast<uint4*>(smem + Sh::kRec + warp * Sh::kPair) + lane;  // (PAIR) operands, 32 lanes each
+    if (second) {
+      named_bar_sync(1 + warp, 64);
+#pragma unroll
+      for (int c = 0; c < DK / 16; ++c) {
+        const uint4 h = pair[c * 32];
+#pragma unroll
+        for (int n = 0; n < 8; n += 2) {
+          uint32_t q[4];
+          ldmatrix_x4(base + Sh::kQ + tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi), q[0], q[1], q[2], q[3]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (c == 0) mma_16816_first<true>(o[n + x], h.x, h.y, h.z, h.w, q[2 * x], q[2 * x + 1]);
+            else mma_16816<true>(o[n + x], h.x, h.y, h.z, h.w, q[2 * x], q[2 * x + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) scale_out(n);
+      named_bar_sync(1 + kWalkWarps + warp, 64);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 x = pair[(DK / 16 + 2 * k) * 32], y = pair[(DK / 16 + 2 * k + 1) * 32];
+        const uint32_t h[4] = {x.x, x.y, x.z, x.w}, l[4] = {y.x, y.y, y.z, y.w};
+        add_pn(k, h, l);
+      }
+      put_out();
+      rec += rec_step;
+      continue;
+    }
     // S0^T k_j and S0^T q_j of the chunk's tokens
-    float r[8][4], o[8][4];
+    float r[8][4];
 #pragma unroll
     for (int c = 0; c < DK / 16; ++c) {
       uint32_t h[4], l[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) split_bf16x2(s[2 * c + (x >> 1)][2 * (x & 1)], s[2 * c + (x >> 1)][2 * (x & 1) + 1], h[x], l[x]);
+      if (PAIR) pair[c * 32] = make_uint4(h[0], h[1], h[2], h[3]);
 #pragma unroll
       for (int n = 0; n < 8; n += 2) {
         uint32_t b[4], q[4];
         const uint32_t at = tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi);
         ldmatrix_x4(base + at, b[0], b[1], b[2], b[3]);
-        ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
+        if (!PAIR) ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
         // (a sum's next product comes four later: it takes about 21 cycles, one issues in 8)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -625,6 +709,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
         // only the output sees the product with q: one bf16 term (2^-9) of the state
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
+          if (PAIR) continue;
           if (c == 0) mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
           else mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
         }
@@ -632,6 +717,7 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
         for (int x = 0; x < 2; ++x) mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
       }
     }
+    if (PAIR) named_bar_arrive(1 + warp, 64);
     // R = v - exp(G) S0^T k; its two terms as A operands over the tokens
     uint32_t rh[4][4] = {}, rl[4][4] = {};
 #pragma unroll
@@ -641,16 +727,12 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float2 e = *reinterpret_cast<const float2*>(f + (n + x) * 8 + 2 * t4);
-        const float2 g = *reinterpret_cast<const float2*>(f + kC + (n + x) * 8 + 2 * t4);
         float* y = r[n + x];
         y[0] = __uint_as_float(v[2 * x] << 16) - e.x * y[0];
         y[1] = __uint_as_float(v[2 * x] & 0xffff0000u) - e.y * y[1];
         y[2] = __uint_as_float(v[2 * x + 1] << 16) - e.x * y[2];
         y[3] = __uint_as_float(v[2 * x + 1] & 0xffff0000u) - e.y * y[3];
-        o[n + x][0] *= g.x;
-        o[n + x][1] *= g.y;
-        o[n + x][2] *= g.x;
-        o[n + x][3] *= g.y;
+        if (!PAIR) scale_out(n + x);
       }
     }
     // the two terms of a 16-token column block of x
@@ -706,36 +788,22 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
     times(one, w + 6, 6, 3, false);
     split(w, 2, rh[2], rl[2]);
     split(w, 3, rh[3], rl[3]);
-    // out += P N
+    if (PAIR) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t b[8][2];
+      for (int k = 0; k < 4; ++k) {
+        pair[(DK / 16 + 2 * k) * 32] = make_uint4(rh[k][0], rh[k][1], rh[k][2], rh[k][3]);
+        pair[(DK / 16 + 2 * k + 1) * 32] = make_uint4(rl[k][0], rl[k][1], rl[k][2], rl[k][3]);
+      }
+      named_bar_arrive(1 + kWalkWarps + warp, 64);
+    } else {
 #pragma unroll
-      for (int n = 2 * k; n < 8; n += 2)
-        ldmatrix_x4(mat + 2 * kRecT + tile_at<128>(n * 8 + mtop * 8 + mrow, 2 * k + mhi), b[n][0], b[n][1], b[n + 1][0], b[n + 1][1]);
-#pragma unroll
-      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[n][0], b[n][1]);
-#pragma unroll
-      for (int n = 2 * k; n < 8; ++n) mma_16816<true>(o[n], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[n][0], b[n][1]);
+      for (int k = 0; k < 4; ++k) add_pn(k, rh[k], rl[k]);
+      __syncthreads();  // every warp is done with the matrices
+      if (t0 + kC < c1) load_matrices(0, rec + rec_step);
+      cp_async_commit();
+      put_out();
     }
-    __syncthreads();  // every warp is done with the matrices
     rec += rec_step;
-    if (t0 + kC < c1) load_matrices(rec);
-    cp_async_commit();
-    // the output's 16 columns of 64 tokens, turned in shared memory: in the place of the
-    // values, which no other warp reads
-#pragma unroll
-    for (int n = 0; n < 8; n += 2)
-      stmatrix_x4_trans(base + Sh::kVAt + tile_at<VR>(n * 8 + mtop * 8 + mrow, 2 * warp + mhi), pack16<true>(o[n][0], o[n][1]),
-                        pack16<true>(o[n][2], o[n][3]), pack16<true>(o[n + 1][0], o[n + 1][1]), pack16<true>(o[n + 1][2], o[n + 1][3]));
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = i * 16 + (lane >> 1);
-      if (t0 + t < c1)
-        *reinterpret_cast<uint4*>(d.out + (t0 + t) * d.out_stride + hv * DV + col + 16 * warp + (lane & 1) * 8) =
-            *reinterpret_cast<const uint4*>(smem + stage * Sh::kStage + Sh::kVAt + tile_at<VR>(t, 2 * warp + (lane & 1)));
-    }
     // S = exp(G_64) S + k (exp(G_64 - G) n)^T
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -771,7 +839,8 @@ __global__ void __launch_bounds__(kWalkThreads, 2) gated_delta_walk_kernel(const
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) S[(n * 8 + 2 * t4 + (x & 1)) * DV + quad + (x >> 1) * 8] = s[n][x];
+    for (int x = 0; x < 4; ++x)
+      if (!second) S[(n * 8 + 2 * t4 + (x & 1)) * DV + quad + (x >> 1) * 8] = s[n][x];
 }
 
 int delta_args(const d3_gated_delta_t* p, int n, int T, int32_t* status, DeltaArgs& a) {
@@ -842,17 +911,13 @@ int launch_prep(const ChunkArgs& a, cudaStream_t s) {
   return check_launch("d3_gated_delta_chunk");
 }
 
-template <int DK, int DV>
+template <int DK, int DV, bool PAIR>
 int launch_walk(const ChunkArgs& a, cudaStream_t s) {
-  // CTAs that fit one to an SM ask for enough shared memory to be placed so: side by
-  // side they take twice as long (2048 tokens of one sequence: 197 against 104 us)
-  constexpr int kAlone = 120 * 1024;
-  static_assert(WalkShape<DK>::kSmem <= kAlone);
+  constexpr int kSmem = WalkShape<DK, PAIR>::kSmem;
   static bool ready[64] = {};
-  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV>, kAlone, ready)) return rc;
-  const dim3 grid(DV / kWalkCols, a.d.value_heads, a.n);
-  const bool alone = static_cast<int64_t>(grid.x) * grid.y * grid.z <= sm_count();
-  launch_kernel(gated_delta_walk_kernel<DK, DV>, grid, dim3(kWalkThreads), alone ? kAlone : WalkShape<DK>::kSmem, s, a);
+  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV, PAIR>, kSmem, ready)) return rc;
+  launch_kernel(gated_delta_walk_kernel<DK, DV, PAIR>, dim3(DV / kWalkCols, a.d.value_heads, a.n), dim3(kWalkThreads * (PAIR ? 2 : 1)),
+                kSmem, s, a);
   return check_launch("d3_gated_delta_chunk");
 }
 
@@ -860,7 +925,11 @@ template <int DK>
 int launch_chunk(const ChunkArgs& a, int dv, cudaStream_t s) {
   if (a.T > 0)
     if (int rc = launch_prep<DK>(a, s)) return rc;
-  return dv == 64 ? launch_walk<DK, 64>(a, s) : launch_walk<DK, 128>(a, s);
+  // pairs of warps where every CTA has an SM of its own (side by side two CTAs would share
+  // one: 2048 tokens of one sequence took 221 us so)
+  const bool alone = static_cast<int64_t>(dv / kWalkCols) * a.d.value_heads * a.n <= sm_count();
+  if (dv == 64) return alone ? launch_walk<DK, 64, true>(a, s) : launch_walk<DK, 64, false>(a, s);
+  return alone ? launch_walk<DK, 128, true>(a, s) : launch_walk<DK, 128, false>(a, s);
 }
 
 }  // namespace
