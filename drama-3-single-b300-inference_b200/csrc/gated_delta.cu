@@ -36,10 +36,10 @@
 // Three terms would cost half as many products again.
 //
 // What bounds it. The state passes from chunk to chunk, so a sequence of 2048 tokens is 32
-// steps of 3.4 us however much of the GPU is free (126 us in all, 113 of them the walk);
-// of a step's 6500 cycles per warp 3360 are tensor (420 products of 8), the rest the
-// splitting, the short dependent products of the solve, and loads and stores. 64
-// ragged prompts of 32 heads (17.5k tokens) take 552 us: the walk 425 at 0.59 of the
+// steps of 3.1 us however much of the GPU is free (118 us in all, 100 of them the walk);
+// of a step's 5800 cycles 2500 are tensor (316 products of 8 in the first warp of a pair),
+// the rest the splitting, the short dependent products of the solve, and their operands. 64
+// ragged prompts of 32 heads (17.5k tokens) take 545 us: the walk 420 at 0.59 of the
 // rate of mma.sync and 0.25 of HBM's, the first kernel 130. tcgen05 was not taken: the
 // state would go through tensor memory and registers five times a chunk (state, R, N and
 // their terms), 500 columns of 32 lanes and about 2000 instructions a thread, as long as
@@ -554,7 +554,7 @@ struct WalkShape {
 // beside it that takes what the next chunk does not wait for, the loads, S0^T q, P N and the
 // output. It gets the state's first terms and N as the A operands they are, through
 // shared memory (two named barriers a chunk). 2048 tokens of one sequence: 126 us without,
-// 106 with. With many CTAs it would only take the place of a second CTA's warps.
+// 118 with. With many CTAs it would only take the place of a second CTA's warps.
 template <int DK, int DV, bool PAIR>
 __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_delta_walk_kernel(const ChunkArgs a) {
   using Sh = WalkShape<DK, PAIR>;
@@ -688,34 +688,45 @@ __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) g
     }
     // S0^T k_j and S0^T q_j of the chunk's tokens
     float r[8][4];
+    // (operands are read one step ahead of their products, and a sum's next product comes
+    // four later: it takes about 21 cycles, one issues in 8)
+    uint32_t kb[2][4], qb[2][4];
+    auto read_kq = [&](int i) {  // step i: 16 columns c of 16 tokens n
+      const uint32_t at = tile_at<DK * 2>((i & 3) * 16 + mtop * 8 + mrow, 2 * (i >> 2) + mhi);
+      ldmatrix_x4(base + at, kb[i & 1][0], kb[i & 1][1], kb[i & 1][2], kb[i & 1][3]);
+      if (!PAIR) ldmatrix_x4(base + Sh::kQ + at, qb[i & 1][0], qb[i & 1][1], qb[i & 1][2], qb[i & 1][3]);
+    };
+    read_kq(0);
+    uint32_t hs[2][4], ls[2][4];
+    auto split_s = [&](int c, int x) {  // a quarter of the state's terms for columns c
+      split_bf16x2(s[2 * c + (x >> 1)][2 * (x & 1)], s[2 * c + (x >> 1)][2 * (x & 1) + 1], hs[c & 1][x], ls[c & 1][x]);
+    };
 #pragma unroll
-    for (int c = 0; c < DK / 16; ++c) {
-      uint32_t h[4], l[4];
+    for (int x = 0; x < 4; ++x) split_s(0, x);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) split_bf16x2(s[2 * c + (x >> 1)][2 * (x & 1)], s[2 * c + (x >> 1)][2 * (x & 1) + 1], h[x], l[x]);
-      if (PAIR) pair[c * 32] = make_uint4(h[0], h[1], h[2], h[3]);
+    for (int i = 0; i < DK / 4; ++i) {
+      const int c = i >> 2, n = (i & 3) * 2;
+      if (i + 1 < DK / 4) read_kq(i + 1);
+      const uint32_t(&h)[4] = hs[c & 1];
+      const uint32_t(&l)[4] = ls[c & 1];
+      if (PAIR && n == 0) pair[c * 32] = make_uint4(h[0], h[1], h[2], h[3]);
+      const uint32_t(&b)[4] = kb[i & 1];
+      const uint32_t(&q)[4] = qb[i & 1];
 #pragma unroll
-      for (int n = 0; n < 8; n += 2) {
-        uint32_t b[4], q[4];
-        const uint32_t at = tile_at<DK * 2>(n * 8 + mtop * 8 + mrow, 2 * c + mhi);
-        ldmatrix_x4(base + at, b[0], b[1], b[2], b[3]);
-        if (!PAIR) ldmatrix_x4(base + Sh::kQ + at, q[0], q[1], q[2], q[3]);
-        // (a sum's next product comes four later: it takes about 21 cycles, one issues in 8)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (c == 0) mma_16816_first<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
-          else mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
-        }
-        // only the output sees the product with q: one bf16 term (2^-9) of the state
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (PAIR) continue;
-          if (c == 0) mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
-          else mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
+      for (int x = 0; x < 2; ++x) {
+        if (c == 0) mma_16816_first<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
+        else mma_16816<true>(r[n + x], h[0], h[1], h[2], h[3], b[2 * x], b[2 * x + 1]);
       }
+      // only the output sees the product with q: one bf16 term (2^-9) of the state
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (PAIR) continue;
+        if (c == 0) mma_16816_first<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+        else mma_16816<true>(o[n + x], h[0], h[1], h[2], h[3], q[2 * x], q[2 * x + 1]);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) mma_16816<true>(r[n + x], l[0], l[1], l[2], l[3], b[2 * x], b[2 * x + 1]);
+      if (c + 1 < DK / 16) split_s(c + 1, i & 3);
     }
     if (PAIR) named_bar_arrive(1 + warp, 64);
     // R = v - exp(G) S0^T k; its two terms as A operands over the tokens
@@ -813,23 +824,29 @@ __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) g
         split_bf16x2(w[2 * k + (x >> 1)][2 * (x & 1)] * e.x, w[2 * k + (x >> 1)][2 * (x & 1) + 1] * e.y, rh[k][x], rl[k][x]);
       }
     const float end = f[3 * kC];
+    uint32_t kt[2][4][2];
+    auto read_k = [&](int i) {  // step i: tokens 16 k .. of 4 columns of 8
+      const int n = (i >> 2) * 4, k = i & 3;
+      uint32_t(&b)[4][2] = kt[i & 1];
 #pragma unroll
-    for (int n = 0; n < DK / 8; n += 4) {
-      float p[4][4];
+      for (int x = 0; x < 4; x += 2)
+        ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + x + mtop), b[x][0], b[x][1], b[x + 1][0], b[x + 1][1]);
+    };
+    read_k(0);
+    float p[4][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t b[4][2];
+    for (int i = 0; i < DK / 8; ++i) {
+      const int n = (i >> 2) * 4, k = i & 3;
+      if (i + 1 < DK / 8) read_k(i + 1);
+      const uint32_t(&b)[4][2] = kt[i & 1];
 #pragma unroll
-        for (int x = 0; x < 4; x += 2)
-          ldmatrix_x4_trans(base + tile_at<DK * 2>(k * 16 + mhi * 8 + mrow, n + x + mtop), b[x][0], b[x][1], b[x + 1][0], b[x + 1][1]);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (k == 0) mma_16816_first<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
-          else mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) mma_16816<true>(p[x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[x][0], b[x][1]);
+      for (int x = 0; x < 4; ++x) {
+        if (k == 0) mma_16816_first<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
+        else mma_16816<true>(p[x], rh[k][0], rh[k][1], rh[k][2], rh[k][3], b[x][0], b[x][1]);
       }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) mma_16816<true>(p[x], rl[k][0], rl[k][1], rl[k][2], rl[k][3], b[x][0], b[x][1]);
+      if (k < 3) continue;
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll

@@ -16,7 +16,7 @@
 // that joins its parts through shared memory, in one launch (unit_ctas).
 //
 // Measured (bf16, 16 query and 2 key heads of 256, pages of 16): 4 sequences of 100k to
-// 131k tokens, 977 MB, in 167 us, 5.84 TB/s or 0.90 of the copy rate (a split of the line
+// 131k tokens, 977 MB, in 162 us, 6.04 TB/s or 0.93 of the copy rate (a split of the line
 // into more CTAs than fit at once, deeper rings and prefetches to L2 were all slower; SMs
 // do not get equal shares of the bandwidth, and the slowest ends the kernel); 64 of up to
 // 2048, 136 MB, in 33 us, of which start and joining take about 10; 1 of 301 in 8.4 us. 16
