@@ -315,20 +315,21 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   float* sB = sG + 2 * kC;       // [2][64]
   float* sRk = sB + 2 * kC;
   float* sRq = sRk + kC;
-  float* sScan = sRq + kC;
-  int* found = reinterpret_cast<int*>(sScan + 4);
+  int* sSeq = reinterpret_cast<int*>(sRq + kC);  // [warps]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
   const DeltaArgs& d = a.d;
   const int hk = blockIdx.y;
   pdl_wait();
   pdl_trigger();
   // the sequence of this record, each thread looking at its own ones
-  if (tid == 0) *found = -1;
-  __syncthreads();
+  int lo = -1;
   for (int i = tid; i < a.n; i += kPrepThreads)
-    if (first_record(max(0, __ldg(a.cu + i)), i) <= blockIdx.x && first_record(max(0, __ldg(a.cu + i + 1)), i + 1) > blockIdx.x) *found = i;
+    if (first_record(max(0, __ldg(a.cu + i)), i) <= blockIdx.x && first_record(max(0, __ldg(a.cu + i + 1)), i + 1) > blockIdx.x) lo = i;
+  lo = __reduce_max_sync(0xffffffffu, lo);
+  if (lane == 0) sSeq[warp] = lo;
   __syncthreads();
-  const int lo = *found;
+#pragma unroll
+  for (int w = 0; w < kPrepThreads / 32; ++w) lo = max(lo, sSeq[w]);
   if (lo < 0) return;
   const int c0 = max(0, __ldg(a.cu + lo)), c1 = min(a.T, __ldg(a.cu + lo + 1));
   const int64_t chunk = static_cast<int64_t>(blockIdx.x) - first_record(c0, lo);
@@ -339,36 +340,38 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   load_rows<DK * 2, kPrepThreads>(kt, d.k + hk * DK, d.k_stride, t0, c1, tid);
   load_rows<DK * 2, kPrepThreads>(qt, d.q + hk * DK, d.q_stride, t0, c1, tid);
   cp_async_commit();
-  // decays and step sizes of the first two heads, on their way meanwhile
-  const int gh = tid >> 6, gt = tid & (kC - 1);  // (threads 0-127) head, token
-  auto fetch = [&](const float* x, int64_t stride, int hv) {
-    return gt < nt && hv < (hk + 1) * d.rep ? __ldg(x + (t0 + gt) * stride + hv) : 0.f;
+  // sums of the decays, and step sizes, of value heads hv0 and hv0 + 1: a warp each, two
+  // tokens per lane
+  auto gates = [&](int hv0) {
+    if (warp >= 2) return;
+    float g[2], be[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int t = 2 * lane + x;
+      const bool in = t < nt && hv0 + warp < (hk + 1) * d.rep;
+      // (a decay to below 2^-126 is 0 either way; the bound keeps later differences exact
+      // and takes g = -infinity, a reset)
+      g[x] = in ? __ldg(d.g + (t0 + t) * d.g_stride + hv0 + warp) * 1.4426950408889634f : 0.f;
+      g[x] = g[x] < -150.f ? -150.f : g[x];
+      be[x] = in ? __ldg(d.beta + (t0 + t) * d.beta_stride + hv0 + warp) : 0.f;
+    }
+    float sum = g[0] + g[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    float before = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane == 0) before = 0.f;
+    *reinterpret_cast<float2*>(sG + warp * kC + 2 * lane) = make_float2(before + g[0], sum);
+    *reinterpret_cast<float2*>(sB + warp * kC + 2 * lane) = make_float2(be[0], be[1]);
   };
-  float g_next = 0.f, b_next = 0.f;
-  if (tid < 2 * kC) {
-    g_next = fetch(d.g, d.g_stride, hk * d.rep + gh);
-    b_next = fetch(d.beta, d.beta_stride, hk * d.rep + gh);
-  }
+  gates(hk * d.rep);  // while the tiles are on their way
   cp_async_wait<0>();
   __syncthreads();
   const int role = warp >> 2, rows = 16 * (warp & 3);
-  // norms: two threads per row of k (warps 0-3) or q
-  {
-    const int r = (tid & 127) >> 1;
-    float xx = 0.f;
-#pragma unroll
-    for (int c = 0; c < DK / 16; ++c) {
-      const uint4 x = *reinterpret_cast<const uint4*>(smem + role * Sh::kTile + tile_at<DK * 2>(r, c * 2 + (tid & 1)));
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) xx = fma_bf16x2_seq(xs[i], xs[i], xx);
-    }
-    xx += __shfl_xor_sync(0xffffffffu, xx, 1);
-    const float f = d.l2norm ? rsqrtf(xx + d.eps) : 1.f;
-    if ((tid & 1) == 0) (role ? sRq : sRk)[r] = r < nt ? (role ? d.scale * f : f) : 0.f;
-  }
-  // products of rows `rows` .. + 15 with the keys up to the diagonal block
-  float acc[8][4];
+  // products of rows `rows` .. + 15 with the keys up to the diagonal block, and the rows' norms
+  float acc[8][4], norm[2] = {};
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -387,36 +390,29 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
       mma_16816<true>(acc[n], x[0], x[1], x[2], x[3], b[0], b[1]);
       mma_16816<true>(acc[n + 1], x[0], x[1], x[2], x[3], b[2], b[3]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) norm[i & 1] = fma_bf16x2_seq(x[i], x[i], norm[i & 1]);  // rows quad, quad + 8
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    norm[i] += __shfl_xor_sync(0xffffffffu, norm[i], 1);
+    norm[i] += __shfl_xor_sync(0xffffffffu, norm[i], 2);
+    const int r = rows + quad + 8 * i;
+    const float f = d.l2norm ? rsqrtf(norm[i] + d.eps) : 1.f;
+    if (t4 == 0) (role ? sRq : sRk)[r] = r < nt ? (role ? d.scale * f : f) : 0.f;
   }
   for (int hv0 = hk * d.rep; hv0 < (hk + 1) * d.rep; hv0 += 2) {
     const int heads = min(2, (hk + 1) * d.rep - hv0);
     uint8_t* rec0 = a.rec + (static_cast<int64_t>(blockIdx.x) * d.value_heads + hv0) * kRecBytes;
-    __syncthreads();  // the tiles, or the previous heads' matrices, are no longer read
-    float G = 0.f;
-    if (tid < 2 * kC) {
-      // (a decay to below 2^-126 is 0 either way; the bound keeps later differences exact
-      // and takes g = -infinity, a reset)
-      G = g_next * 1.4426950408889634f;
-      G = G < -150.f ? -150.f : G;
-      sB[tid] = b_next;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float y = __shfl_up_sync(0xffffffffu, G, o);
-        if (lane >= o) G += y;
-      }
-      if (lane == 31) sScan[warp] = G;
-      g_next = fetch(d.g, d.g_stride, hv0 + 2 + gh);
-      b_next = fetch(d.beta, d.beta_stride, hv0 + 2 + gh);
+    if (hv0 > hk * d.rep) {
+      __syncthreads();  // the previous heads' are no longer read
+      gates(hv0);
     }
-    __syncthreads();
-    if (tid < 2 * kC) {
-      if (warp & 1) G += sScan[warp - 1];
-      sG[tid] = G;
-    }
-    __syncthreads();
-    if (tid < 2 * kC && gh < heads) {
+    __syncthreads();  // nor are the tiles
+    const int gh = tid >> 6, gt = tid & (kC - 1);  // (threads 0-127) head, token
+    if (gh < heads) {
       float* f = reinterpret_cast<float*>(rec0 + gh * kRecBytes + kRecScal);
-      const float end = sG[gh * kC + kC - 1];
+      const float G = sG[gh * kC + gt], end = sG[gh * kC + kC - 1];
       f[gt] = exp2_fast(G) * sRk[gt];
       f[kC + gt] = exp2_fast(G) * sRq[gt];
       f[2 * kC + gt] = exp2_fast(end - G) * sRk[gt];
