@@ -36,11 +36,11 @@
 // Three terms would cost half as many products again.
 //
 // What bounds it. The state passes from chunk to chunk, so a sequence of 2048 tokens is 32
-// steps of 3.1 us however much of the GPU is free (118 us in all, 100 of them the walk);
-// of a step's 5800 cycles 2500 are tensor (316 products of 8 in the first warp of a pair),
+// steps of 2.4 us however much of the GPU is free (92 us in all, 75 of them the walk);
+// of a step's 4400 cycles 2500 are tensor (316 products of 8 in the first warp of a pair),
 // the rest the splitting, the short dependent products of the solve, and their operands. 64
-// ragged prompts of 32 heads (17.5k tokens) take 545 us: the walk 420 at 0.59 of the
-// rate of mma.sync and 0.25 of HBM's, the first kernel 130. tcgen05 was not taken: the
+// ragged prompts of 32 heads (17.5k tokens) take 537 us: the walk 413 at 0.60 of the
+// rate of mma.sync and 0.33 of HBM's, the first kernel 124. tcgen05 was not taken: the
 // state would go through tensor memory and registers five times a chunk (state, R, N and
 // their terms), 500 columns of 32 lanes and about 2000 instructions a thread, as long as
 // the walk takes now at a few percent of that unit.
@@ -212,21 +212,18 @@ struct ChunkArgs {
   int T, n;
 };
 
-// Copies rows [t0, t0 + 64) (zeros from t1 on) of BYTES bytes each into a tile. A
-// thread's rows are THREADS / PIECES apart (a multiple of 8), so its piece of a row and
-// the permutation of the pieces are the same in all of them.
+// Copies rows [t0, t0 + 64) (zeros from t1 on) of BYTES bytes each into a tile, by
+// THREADS threads of which this is number `thread`.
 template <int BYTES, int THREADS>
 __device__ __forceinline__ void load_rows(uint32_t tile, const __nv_bfloat16* src, int64_t stride, int t0, int t1, int thread) {
   constexpr int PIECES = BYTES / 16, STEP = THREADS / PIECES;
-  static_assert(STEP % 8 == 0);
   const int r = thread / PIECES, c = thread % PIECES;
   const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (t0 + r) * stride) + c * 16;
-  const uint32_t to = tile + tile_at<BYTES>(r, c);
   const int64_t step = STEP * stride * 2;
 #pragma unroll
   for (int i = 0; i < kC / STEP; ++i, row += step) {
     const bool take = t0 + r + i * STEP < t1;  // past the end nothing is read
-    cp_async_16_zfill(to + i * STEP * BYTES, take ? row : reinterpret_cast<const uint8_t*>(src), take);
+    cp_async_16_zfill(tile + tile_at<BYTES>(r + i * STEP, c), take ? row : reinterpret_cast<const uint8_t*>(src), take);
   }
 }
 
@@ -300,7 +297,7 @@ __device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int head
 }
 
 // One CTA per (record, key head), two of its value heads at a time: bound by latency and
-// instructions, not by its 279 MB (138 us for 305 chunks of 16 key heads, 43% of issue
+// instructions, not by its 278 MB (124 us for 305 chunks of 16 key heads, 45% of issue
 // slots busy with four CTAs on an SM). Warps 0-3 make
 // k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads share them.
 template <int DK>
@@ -522,23 +519,21 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   }
 }
 
-constexpr int kWalkWarps = 4, kWalkThreads = kWalkWarps * 32, kWalkCols = 16 * kWalkWarps;
-
 // Shared memory: keys, queries, values and factors of two chunks, and T and P of one, whose
 // place is free again by the time the state is updated, so that two CTAs share an SM. With
-// PAIR (below) T and P of two, and what the warps of a pair hand over.
-template <int DK, bool PAIR>
+// PAIR (below) T and P of two, and what the warps of a pair hand over. W: warps of columns.
+template <int DK, bool PAIR, int W>
 struct WalkShape {
-  static constexpr int kKT = kC * DK * 2, kV = kC * kWalkCols * 2;
+  static constexpr int kKT = kC * DK * 2, kV = kC * W * 32;
   static constexpr int kQ = kKT, kVAt = 2 * kKT, kF = kVAt + kV, kMat = kF + 1024;
   static constexpr int kStage = kMat + (PAIR ? 3 * kRecT : 0);
   static constexpr int kRec = 2 * kStage;  // the matrices, or the pairs' places
   static constexpr int kPairS = DK / 16 * 512, kPair = kPairS + 8 * 512;
-  static constexpr int kSmem = kRec + (PAIR ? kWalkWarps * kPair : 3 * kRecT);
+  static constexpr int kSmem = kRec + (PAIR ? W * kPair : 3 * kRecT);
   static_assert(kSmem <= (PAIR ? 227 : 113) * 1024);
 };
 
-// One CTA per (64 value columns, value head, sequence) walks the sequence's
+// One CTA per (16 W value columns, value head, sequence) walks the sequence's
 // chunks. Warp w holds the transposed state of its 16 value columns, [16, DK], as
 // mma accumulators: these are laid out like A operands, so the state, R and N go from
 // product to product in registers, and warps share only what they read (keys,
@@ -549,29 +544,30 @@ struct WalkShape {
 // PAIR, for few CTAs, where a chunk's latency is what counts: each warp has a second one
 // beside it that takes what the next chunk does not wait for, the loads, S0^T q, P N and the
 // output. It gets the state's first terms and N as the A operands they are, through
-// shared memory (two named barriers a chunk). 2048 tokens of one sequence: 126 us without,
-// 118 with. With many CTAs it would only take the place of a second CTA's warps.
-template <int DK, int DV, bool PAIR>
-__global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_delta_walk_kernel(const ChunkArgs a) {
-  using Sh = WalkShape<DK, PAIR>;
-  constexpr int VR = kWalkCols * 2, THREADS = kWalkThreads * (PAIR ? 2 : 1);
+// shared memory (two named barriers a chunk). 2048 tokens of one sequence: 125 us without, 118
+// with 64 columns, 92 with 32, where each warp has a scheduler and its tensor unit to itself.
+// With many CTAs it would only take the place of a second CTA's warps.
+template <int DK, int DV, bool PAIR, int W>
+__global__ void __launch_bounds__(32 * W * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_delta_walk_kernel(const ChunkArgs a) {
+  using Sh = WalkShape<DK, PAIR, W>;
+  constexpr int VR = W * 32, LOADERS = 32 * W, THREADS = LOADERS * (PAIR ? 2 : 1);
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, quad = lane >> 2, t4 = lane & 3;
-  const int warp = (tid >> 5) & (kWalkWarps - 1);        // its 16 columns
-  const bool second = PAIR && tid >= kWalkThreads;     // the pair's second warp
+  const int warp = (tid >> 5) & (W - 1);      // its 16 columns
+  const bool second = PAIR && tid >= LOADERS;  // the pair's second warp
   const bool loads = !PAIR || second;
-  const int lt = PAIR ? tid - kWalkThreads : tid;        // number among those that load
+  const int lt = PAIR ? tid - LOADERS : tid;     // number among those that load
   const int mrow = lane & 7, mhi = (lane >> 3) & 1, mtop = lane >> 4;
   const DeltaArgs& d = a.d;
   const int seq = blockIdx.z, hv = blockIdx.y, hk = hv / d.rep;
-  const int col = blockIdx.x * kWalkCols;  // first value column of the CTA
+  const int col = blockIdx.x * 16 * W;  // first value column of the CTA
   pdl_wait();
   pdl_trigger();
   const int c0 = max(0, __ldg(a.cu + seq)), c1 = min(a.T, __ldg(a.cu + seq + 1));
   const int slot = delta_slot(d, seq);
   if (slot < 0) {
-    for (int e = tid; e < (c1 - c0) * (kWalkCols / 8); e += THREADS)
-      *reinterpret_cast<uint4*>(d.out + (c0 + e / (kWalkCols / 8)) * d.out_stride + hv * DV + col + e % (kWalkCols / 8) * 8) = make_uint4(0, 0, 0, 0);
+    for (int e = tid; e < (c1 - c0) * (2 * W); e += THREADS)
+      *reinterpret_cast<uint4*>(d.out + (c0 + e / (2 * W)) * d.out_stride + hv * DV + col + e % (2 * W) * 8) = make_uint4(0, 0, 0, 0);
     return;
   }
   const uint8_t* rec = a.rec + (first_record(c0, seq) * d.value_heads + hv) * kRecBytes;
@@ -579,16 +575,16 @@ __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) g
   const uint32_t sm = smem_u32(smem);
   auto load_tokens = [&](int stage, int t0, const uint8_t* rec) {
     const uint32_t s = sm + stage * Sh::kStage;
-    load_rows<DK * 2, kWalkThreads>(s, d.k + hk * DK, d.k_stride, t0, c1, lt);
-    load_rows<DK * 2, kWalkThreads>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1, lt);
-    load_rows<VR, kWalkThreads>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1, lt);
+    load_rows<DK * 2, LOADERS>(s, d.k + hk * DK, d.k_stride, t0, c1, lt);
+    load_rows<DK * 2, LOADERS>(s + Sh::kQ, d.q + hk * DK, d.q_stride, t0, c1, lt);
+    load_rows<VR, LOADERS>(s + Sh::kVAt, d.v + hv * DV + col, d.v_stride, t0, c1, lt);
     if (lt < 49) cp_async_16(smem + stage * Sh::kStage + Sh::kF + lt * 16, rec + kRecScal + lt * 16);
   };
   auto load_matrices = [&](int stage, const uint8_t* rec) {  // blocks up to the diagonal
     uint8_t* to = smem + (PAIR ? stage * Sh::kStage + Sh::kMat : Sh::kRec);
 #pragma unroll
-    for (int i = 0; i < 3 * kC * 8 / kWalkThreads; ++i) {
-      const int e = i * kWalkThreads + lt, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
+    for (int i = 0; i < 3 * kC * 8 / LOADERS; ++i) {
+      const int e = i * LOADERS + lt, r = (e >> 3) & (kC - 1), c = e & 7, m = e / (kC * 8);
       if (c < (r >> 4) * 2 + 2) cp_async_16(to + m * kRecT + tile_at<128>(r, c), rec + m * kRecT + r * 128 + c * 16);
     }
   };
@@ -671,7 +667,7 @@ __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) g
       }
 #pragma unroll
       for (int n = 0; n < 8; ++n) scale_out(n);
-      named_bar_sync(1 + kWalkWarps + warp, 64);
+      named_bar_sync(1 + W + warp, 64);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint4 x = pair[(DK / 16 + 2 * k) * 32], y = pair[(DK / 16 + 2 * k + 1) * 32];
@@ -801,7 +797,7 @@ __global__ void __launch_bounds__(kWalkThreads * (PAIR ? 2 : 1), PAIR ? 1 : 2) g
         pair[(DK / 16 + 2 * k) * 32] = make_uint4(rh[k][0], rh[k][1], rh[k][2], rh[k][3]);
         pair[(DK / 16 + 2 * k + 1) * 32] = make_uint4(rl[k][0], rl[k][1], rl[k][2], rl[k][3]);
       }
-      named_bar_arrive(1 + kWalkWarps + warp, 64);
+      named_bar_arrive(1 + W + warp, 64);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) add_pn(k, rh[k], rl[k]);
@@ -924,25 +920,31 @@ int launch_prep(const ChunkArgs& a, cudaStream_t s) {
   return check_launch("d3_gated_delta_chunk");
 }
 
-template <int DK, int DV, bool PAIR>
+template <int DK, int DV, bool PAIR, int W>
 int launch_walk(const ChunkArgs& a, cudaStream_t s) {
-  constexpr int kSmem = WalkShape<DK, PAIR>::kSmem;
+  constexpr int kSmem = WalkShape<DK, PAIR, W>::kSmem;
   static bool ready[64] = {};
-  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV, PAIR>, kSmem, ready)) return rc;
-  launch_kernel(gated_delta_walk_kernel<DK, DV, PAIR>, dim3(DV / kWalkCols, a.d.value_heads, a.n), dim3(kWalkThreads * (PAIR ? 2 : 1)),
+  if (int rc = allow_smem(gated_delta_walk_kernel<DK, DV, PAIR, W>, kSmem, ready)) return rc;
+  launch_kernel(gated_delta_walk_kernel<DK, DV, PAIR, W>, dim3(DV / (16 * W), a.d.value_heads, a.n), dim3(32 * W * (PAIR ? 2 : 1)),
                 kSmem, s, a);
   return check_launch("d3_gated_delta_chunk");
+}
+
+template <int DK, int DV>
+int launch_walks(const ChunkArgs& a, cudaStream_t s) {
+  // pairs of warps where every CTA has an SM of its own, with half the columns where
+  // that still holds, so that no two warps of a CTA share a scheduler
+  const int64_t heads = static_cast<int64_t>(a.d.value_heads) * a.n;
+  if (heads * (DV / 32) <= sm_count()) return launch_walk<DK, DV, true, 2>(a, s);
+  if (heads * (DV / 64) <= sm_count()) return launch_walk<DK, DV, true, 4>(a, s);
+  return launch_walk<DK, DV, false, 4>(a, s);
 }
 
 template <int DK>
 int launch_chunk(const ChunkArgs& a, int dv, cudaStream_t s) {
   if (a.T > 0)
     if (int rc = launch_prep<DK>(a, s)) return rc;
-  // pairs of warps where every CTA has an SM of its own (side by side two CTAs would share
-  // one: 2048 tokens of one sequence took 221 us so)
-  const bool alone = static_cast<int64_t>(dv / kWalkCols) * a.d.value_heads * a.n <= sm_count();
-  if (dv == 64) return alone ? launch_walk<DK, 64, true>(a, s) : launch_walk<DK, 64, false>(a, s);
-  return alone ? launch_walk<DK, 128, true>(a, s) : launch_walk<DK, 128, false>(a, s);
+  return dv == 64 ? launch_walks<DK, 64>(a, s) : launch_walks<DK, 128>(a, s);
 }
 
 }  // namespace

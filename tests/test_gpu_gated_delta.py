@@ -77,6 +77,15 @@ def test_chunk(shape, lens):
         assert R.rel_l2(state[i], ws[i]) <= STATE_TOL
 
 
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("n", [14, 26, 60, 100])
+def test_chunk_batches(shape, n):
+    """Numbers of sequences on both sides of where the split over the SMs changes."""
+    out, want, state, ws, status = chunk([(37 * i + 11) % 150 for i in range(n)], shape, seed=n)
+    assert status == 0
+    assert R.rel_l2(out, want) <= OUT_TOL and R.rel_l2(state, ws) <= STATE_TOL
+
+
 @pytest.mark.parametrize("decay", [0.0, 0.01, 30.0])
 def test_chunk_decays(decay):
     """No decay, slow decay, and one that leaves nothing of a state."""
