@@ -235,9 +235,13 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
   constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kSlots, P = Sh::kAhead, ROWS = Sh::kRows;
   constexpr int KS = D / 16, MT = NK / 16, NH = ROWS / 8;
-  constexpr int PIECES = RB / 16, JW = Sh::kJoinWarps, JP = Sh::kJoinPitch;
+  constexpr int PIECES = RB / 16, JW = LINE ? Sh::kJoinWarps : kAttnWarps, JP = Sh::kJoinPitch;
   extern __shared__ __align__(1024) uint8_t smem[];
-  float* join = reinterpret_cast<float*>(smem + Sh::kRing);
+  // without a line a CTA joins once, when its ring is empty: all warps' rows fit there,
+  // and behind them the record for the cluster
+  float* join = reinterpret_cast<float*>(smem + (LINE ? Sh::kRing : 0));
+  constexpr int kRecordAt = kAttnWarps * 8 * JP * 4;
+  static_assert(kRecordAt + Sh::kRecord * 4 <= Sh::kRing);
   uint8_t* qs = smem + Sh::kRing + Sh::kJoin;
   float* stat = reinterpret_cast<float*>(qs + Sh::kQ);  // [warps][2][16]
   int* scratch = reinterpret_cast<int*>(stat + kAttnWarps * 32);
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   float m[NH][2], l[NH][2];  // of heads 2 t4 and 2 t4 + 1
   float lg[NH][2];         // their logits in units of log2, per product
   bool opened = false, whole = false;
-  float* shared_rec = reinterpret_cast<float*>(smem);
+  float* shared_rec = reinterpret_cast<float*>(smem + kRecordAt);
   const int unit0 = cur.unit, b0 = cur.b;
   const bool empty = cur.at >= end;
   int seg_slot = 0, use = 0;
@@ -577,6 +581,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
     if (last || !more) {
       // join the warps: (max, sum) and output rows through shared memory
       opened = false;
+      if (!LINE) cp_async_wait<0>();  // nothing is on its way to the ring any more
       if (more) fetch_q(nxt);
 #pragma unroll
       for (int h = 0; h < NH; ++h)
@@ -593,11 +598,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
       __syncthreads();
       whole = whole && last && (LINE || a.share < 2);
       float* rec = a.partial + (static_cast<int64_t>(blockIdx.x) * 2 + seg_slot) * Sh::kRecord;
-      if (!LINE && a.share > 1) {  // for the cluster: over the ring, which nothing is on its way to any more
-        cp_async_wait<0>();
-        __syncthreads();
-        rec = shared_rec;
-      }
+      if (!LINE) rec = shared_rec;
       const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
       // each warp scales its rows to the common maximum; JW at a time they are
       // added into JW buffers, in the order of the warps
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   const int head = unit0 / a.parts, h0 = head * a.group + (unit0 % a.parts) * ROWS;
   const int nh = min(ROWS, (head + 1) * a.group - h0);
   const float vsc = a.v_scale ? __ldg(a.v_scale + head) : 1.0f;
-  const uint32_t rec = smem_u32(smem);
+  const uint32_t rec = smem_u32(shared_rec);
   for (int e = tid * 4; e < ((nh - rank + a.share - 1) / a.share) * D; e += kAttnThreads * 4) {
     const int r = rank + e / D * a.share, d = e % D;
     float top = -INFINITY, sum = 0.f, x[4] = {};
