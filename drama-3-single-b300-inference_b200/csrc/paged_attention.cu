@@ -19,8 +19,8 @@
 // 131k tokens, 977 MB, in 162 us, 6.04 TB/s or 0.93 of the copy rate (a split of the line
 // into more CTAs than fit at once, deeper rings and prefetches to L2 were all slower; SMs
 // do not get equal shares of the bandwidth, and the slowest ends the kernel); 64 of up to
-// 2048, 136 MB, in 33 us, of which start and joining take about 10; 1 of 301 in 8.4 us. 16
-// of up to 16411 in e4m3 (32 query and 8 key heads of 128), 311 MB: 64 us, 4.8 TB/s, issue
+// 2048, 136 MB, in 33 us, of which start and joining take about 10; 1 of 301 in 7.1 us. 16
+// of up to 16411 in e4m3 (32 query and 8 key heads of 128), 311 MB: 63 us, 4.9 TB/s, issue
 // slots 0.53 busy with widening and twice the products per byte.
 //
 // Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
@@ -707,31 +707,29 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   if (a.share > 1) cluster_sync();  // no CTA's shared memory goes away while another reads it
 }
 
-constexpr int kGatherWarps = 8, kGatherThreads = kGatherWarps * 32;
-
 // One CTA per query row: rows without keys get zeros, rows of units that several
 // CTAs shared are joined from their records. Groups of D / 4 threads add up every
-// (kGatherThreads * 4 / D)-th record, so the loads of a long unit's records overlap; the
+// (32 WARPS * 4 / D)-th record, so the loads of a long unit's records overlap; the
 // groups are then added in order.
-template <int DT, int D, bool WIDE>
-__global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(const AttnArgs a) {
+template <int DT, int D, bool WIDE, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) paged_attention_join_kernel(const AttnArgs a) {
   using Sh = AttnShape<DT, D, WIDE>;
   constexpr bool QBF16 = DT != D3_DTYPE_F16;
-  constexpr int ROWS = Sh::kRows, LANES = D / 4, GROUPS = kGatherThreads / LANES;
+  constexpr int ROWS = Sh::kRows, THREADS = 32 * WARPS, LANES = D / 4, GROUPS = THREADS / LANES;
   extern __shared__ __align__(1024) uint8_t smem[];
   float4* acc = reinterpret_cast<float4*>(smem);                       // [GROUPS][LANES]
-  float* fac = reinterpret_cast<float*>(smem) + kGatherThreads * 4;      // [a.grid] maximum, then weight
+  float* fac = reinterpret_cast<float*>(smem) + THREADS * 4;      // [a.grid] maximum, then weight
   float* red = fac + a.grid;                                           // [2][warps]
-  int* scratch = reinterpret_cast<int*>(red + 2 * kGatherWarps);
-  int* found = scratch + kGatherWarps;
+  int* scratch = reinterpret_cast<int*>(red + 2 * WARPS);
+  int* found = scratch + WARPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int b = blockIdx.x / a.q_heads, h = blockIdx.x % a.q_heads;
   const int head = h / a.group, part = (h - head * a.group) / ROWS, r = (h - head * a.group) % ROWS;
   const int unit = head * a.parts + part;
-  const int per = (a.B + kGatherThreads - 1) / kGatherThreads;
+  const int per = (a.B + THREADS - 1) / THREADS;
   pdl_trigger();
   int mine, before, total;
-  line_scan<Sh::kTile, kGatherWarps>(a, per, scratch, mine, before, total);
+  line_scan<Sh::kTile, WARPS>(a, per, scratch, mine, before, total);
   const int tiles = seq_tiles<Sh::kTile>(a, b);
   if (b / per == tid) {
     int at = before;
@@ -751,7 +749,7 @@ __global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(co
   const float* rec = a.partial + static_cast<int64_t>(c0) * 2 * Sh::kRecord;  // + 2 c records, c > 0
   auto record = [&](int c) { return c == 0 ? rec0 : rec + static_cast<int64_t>(c) * 2 * Sh::kRecord; };
   float top = -INFINITY, sum = 0.f;
-  for (int c = tid; c < n; c += kGatherThreads) {
+  for (int c = tid; c < n; c += THREADS) {
     const float m = __ldcg(record(c) + ROWS * D + r);
     fac[c] = m;
     top = fmaxf(top, m);
@@ -760,16 +758,16 @@ __global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(co
   if (lane == 0) red[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kGatherWarps; ++w) top = fmaxf(top, red[w]);
+  for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red[w]);
   const float base = top == -INFINITY ? 0.f : top;
-  for (int c = tid; c < n; c += kGatherThreads) {
+  for (int c = tid; c < n; c += THREADS) {
     const float f = exp2f(fac[c] - base);
     fac[c] = f;
     sum += f * __ldcg(record(c) + ROWS * D + ROWS + r);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red[kGatherWarps + warp] = sum;
+  if (lane == 0) red[WARPS + warp] = sum;
   __syncthreads();
   const int d = tid % LANES, g = tid / LANES;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -788,7 +786,7 @@ __global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(co
   float out[4] = {};
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kGatherWarps; ++w) sum += red[kGatherWarps + w];
+  for (int w = 0; w < WARPS; ++w) sum += red[WARPS + w];
   for (int i = 0; i < GROUPS; ++i) {
     const float4 y = acc[i * LANES + d];
     out[0] += y.x;
@@ -800,10 +798,10 @@ __global__ void __launch_bounds__(kGatherThreads) paged_attention_join_kernel(co
 }
 
 // How units of up to `tiles` tiles each are taken: by clusters of the returned number of
-// CTAs (1: whole), or 0: all units' tiles as one line. Measured on 64-tile steps (bf16, 2
-// key heads of 256, us whole / cluster / line): 1 sequence of 256 tokens 10.6 / 8.3 / 9.1,
-// of 1024 27.9 / 10.4 / 10.8; 64 sequences of up to 256 11.4 / 11.9 / 13.4, of up to 1024
-// 30.7 / - / 23.6.
+// CTAs (1: whole), or 0: all units' tiles as one line. Measured in us (bf16, 2 key heads of
+// 256, tiles of 64): 1 sequence of 256 tokens by a cluster 7.0, as a line 9.1, of 1024 9.0
+// and 10.8; 64 sequences of up to 256 whole 10.1, as a line 13.4, of up to 1024 as a line
+// 23.4, whole about 30.
 int unit_ctas(int tiles, int64_t units, int grid) {
   if (tiles <= 2 || (tiles <= 6 && units * 4 >= grid)) return 1;  // short, or enough of them to fill the GPU
   int n = 8;
@@ -843,8 +841,14 @@ int launch_attention(AttnArgs& a, cudaStream_t s) {
     return check_launch("d3_paged_attention");
   }
   launch_kernel(paged_attention_kernel<DT, D, WIDE, true>, dim3(a.grid), dim3(kAttnThreads), Sh::kSmem, s, a);
-  launch_kernel(paged_attention_join_kernel<DT, D, WIDE>, dim3(static_cast<unsigned>(a.B * a.q_heads)), dim3(kGatherThreads),
-                kGatherThreads * 16 + (a.grid + 3 * kGatherWarps + 1) * 4, s, a);
+  // 256 threads a row where they fit at once, 128 for more rows (4 long sequences 162 us
+  // against 167; 200 short ones 38 against 35)
+  const unsigned rows = static_cast<unsigned>(a.B * a.q_heads);
+  const size_t smem = (a.grid + 25) * 4;
+  if (rows <= 8u * sm_count())
+    launch_kernel(paged_attention_join_kernel<DT, D, WIDE, 8>, dim3(rows), dim3(256), 256 * 16 + smem, s, a);
+  else
+    launch_kernel(paged_attention_join_kernel<DT, D, WIDE, 4>, dim3(rows), dim3(128), 128 * 16 + smem, s, a);
   return check_launch("d3_paged_attention");
 }
 
