@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(32 * W * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_d
   const int c0 = max(0, __ldg(a.cu + seq)), c1 = min(a.T, __ldg(a.cu + seq + 1));
   const int slot = delta_slot(d, seq);
   if (slot < 0) {
-    for (int e = tid; e < (c1 - c0) * (2 * W); e += THREADS)
+    for (int64_t e = tid; e < static_cast<int64_t>(c1 - c0) * (2 * W); e += THREADS)
       *reinterpret_cast<uint4*>(d.out + (c0 + e / (2 * W)) * d.out_stride + hv * DV + col + e % (2 * W) * 8) = make_uint4(0, 0, 0, 0);
     return;
   }

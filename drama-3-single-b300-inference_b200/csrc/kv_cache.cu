@@ -154,6 +154,7 @@ extern "C" int d3_kv_append(const void* k, int64_t k_token_stride, int64_t k_hea
   D3_REQUIRE(dtype == (fp8 ? D3_DTYPE_BF16 : cache->dtype), "rows of dtype %d for a cache of dtype %d",
              dtype, cache->dtype);
   D3_REQUIRE(T >= 0, "negative token count");
+  D3_REQUIRE(T <= 0x7fffff00, "too many tokens for one call");  // a CTA's last warps may pass T
   if (T == 0) return D3_OK;
   D3_REQUIRE(k && v && pos && cache->table && cache->k && cache->v, "NULL operand");
   D3_REQUIRE(aligned(k, 16) && aligned(v, 16) && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
@@ -202,6 +203,8 @@ extern "C" int d3_copy_pages(void* pool, int planes, int64_t plane_stride, int p
   D3_REQUIRE(planes >= 0 && pages >= 0 && page_bytes >= 0 && n >= 0, "negative size");
   D3_REQUIRE(pages <= 1 || page_stride >= page_bytes || page_stride <= -page_bytes,
              "pages overlap: page_stride is smaller than a page");
+  // the kernel's counters pass the last plane and pair by up to 65535
+  D3_REQUIRE(planes <= 0x40000000 && n <= 0x40000000, "too many planes or pairs for one call");
   if (planes == 0 || n == 0 || page_bytes == 0 || pages == 0) return D3_OK;
   D3_REQUIRE(pool && src && dst, "NULL operand");
   CopyArgs a{static_cast<uint8_t*>(pool), plane_stride, page_stride, page_bytes, src, dst, pages, status};

@@ -935,7 +935,8 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   D3_REQUIRE(aligned(q, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0, "rows of q must be 16-byte aligned");
   D3_REQUIRE(aligned(out, 8) && out_row_stride % 4 == 0 && out_head_stride % 4 == 0, "rows of out must be 8-byte aligned");
   // the line of tiles (64 keys at least, see AttnShape) is counted in 32 bits
-  D3_REQUIRE(static_cast<int64_t>(B) * a.units * (a.max_len / 64 + 2) < 0x40000000 &&
+  // (and a token's number in a tile that passes the end of its sequence likewise)
+  D3_REQUIRE(a.max_len <= 0x7fffff00 && static_cast<int64_t>(B) * a.units * (a.max_len / 64 + 2) < 0x40000000 &&
                  static_cast<int64_t>(B) * q_heads <= 0x7fffffff,
              "batch, heads and length are too large for one call");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

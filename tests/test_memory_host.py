@@ -90,6 +90,26 @@ def test_c_abi_refuses_bad_arguments():
     assert delta(n=0) == 0
 
 
+def test_c_abi_refuses_sizes_whose_counters_would_pass_32_bits():
+    from d3moe import _lib
+    lib = _lib.load()
+    top = 2**31 - 1
+
+    def refused(rc, text):
+        assert rc == _lib.D3_EINVAL and text in lib.d3_last_error_string(), lib.d3_last_error_string()
+
+    # pages of 2^20 tokens: a table of 2048 of them reaches 2^31
+    c = _lib.D3KvCache(k=4096, v=4096, k_page_stride=0, k_token_stride=0, k_head_stride=64, v_page_stride=0, v_token_stride=0,
+                       v_head_stride=64, table=4096, table_stride=2048, sequences=1, table_pages=2048, num_pages=1,
+                       page_size=1 << 20, heads=1, dim=64, dtype=_lib.D3_DTYPE_BF16)
+    refused(lib.d3_paged_attention(4096, 64, 64, _lib.D3_DTYPE_BF16, 1, 1, ctypes.byref(c), 4096, top, 0, 1.0, 4096, 64, 64,
+                                   None, 4096, 1 << 30, None, None), b"too large for one call")
+    refused(lib.d3_kv_append(4096, 64, 64, 4096, 64, 64, _lib.D3_DTYPE_BF16, top, None, 4096, ctypes.byref(c), None, None),
+            b"too many tokens")
+    refused(lib.d3_copy_pages(4096, 1, 0, 8, 4096, 4096, 4096, 4096, top, None, None), b"too many planes or pairs")
+    refused(lib.d3_copy_pages(4096, top, 0, 8, 4096, 4096, 4096, 4096, 1, None, None), b"too many planes or pairs")
+
+
 def test_python_functions_refuse_cpu_tensors_and_other_things():
     from d3moe import attention, cache, gated_delta
     c, i = torch.zeros((2, 16, 2, 64), dtype=BF16), torch.zeros((1, 2), dtype=torch.int32)
