@@ -32,7 +32,11 @@
 // one movmatrix each. tcgen05 has nothing to add: its tile of 128 rows of keys per
 // instruction would need 8 columns at most, and the operands' way through shared
 // memory is the same. bf16 probabilities go in two terms (2^-17), so the output is
-// rounded once, at its end.
+// rounded once, at its end. f16 ones (f16 and e4m3 caches) go in one term, 2^-11 of
+// themselves: exp2(s - m) times 2^14, which f16 holds, so this is so down to 2^-28 of the
+// warp's largest and off by 2^-39 of that below. (Unscaled they lose bits from 2^-14 on and
+// are 0 from 2^-25 on, while the sum still counts them: a row of many small probabilities
+// beside one key with a small value comes out too small.)
 //
 // An e4m3 cache is widened to f16 in registers (exact). Its queries are scaled by
 // a power of two per row into f16's range (exact for every element within 2^-14
@@ -235,6 +239,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   constexpr bool QBF16 = DT != D3_DTYPE_F16;        // type of q and out
   constexpr int NK = Sh::kNK, RB = Sh::kRowBytes, S = Sh::kSlots, P = Sh::kAhead, ROWS = Sh::kRows;
   constexpr int KS = D / 16, MT = NK / 16, NH = ROWS / 8;
+  constexpr float PS = BF16 ? 1.f : 16384.f;        // the probabilities' factor in the products with V
   constexpr int PIECES = RB / 16, JW = LINE ? Sh::kJoinWarps : kAttnWarps, JP = Sh::kJoinPitch;
   extern __shared__ __align__(1024) uint8_t smem[];
   // without a line a CTA joins once, when its ring is empty: all warps' rows fit there,
@@ -374,7 +379,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
   __syncthreads();
 
   uint32_t qf[KS][NH][2];  // queries as B operands: a column per head
-  float o[KS][NH][4];      // 16 columns of V by 8 heads each
+  float o[KS][NH][4];      // 16 columns of V by 8 heads each, times PS
   float m[NH][2], l[NH][2];  // of heads 2 t4 and 2 t4 + 1
   float lg[NH][2];         // their logits in units of log2, per product
   bool opened = false, whole = false;
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
           const float p0 = exp2f(s[r][h][2 * y] - base[0]), p1 = exp2f(s[r][h][2 * y + 1] - base[1]);
           l[h][0] += p0;
           l[h][1] += p1;
-          const uint32_t hi = pack16<BF16>(p0, p1);
+          const uint32_t hi = pack16<BF16>(p0 * PS, p1 * PS);
           pb[r][h][y] = movmatrix_trans(hi);  // a key's row of heads becomes a head's column of keys
           if constexpr (BF16)
             pl[r][h][y] = movmatrix_trans(pack16<true>(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u)));
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
               float top = -INFINITY;
 #pragma unroll
               for (int y = 0; y < kAttnWarps; ++y) top = fmaxf(top, stat[y * 32 + 8 * w + 2 * t4 + x]);
-              f[x] = exp2f(m[w][x] - (top == -INFINITY ? 0.f : top));
+              f[x] = exp2f(m[w][x] - (top == -INFINITY ? 0.f : top)) * (1.f / PS);
             }
             float* row = join + ((warp % JW) * 8 + 2 * t4) * JP;
 #pragma unroll
