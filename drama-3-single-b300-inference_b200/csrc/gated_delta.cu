@@ -235,28 +235,32 @@ struct PrepShape {
   static constexpr int kMat = kC * kLd * 4;
   static constexpr int kT = 2 * kMat + 2 * 32 * 20 * 4;  // two heads' T and 16 x 16 products, over the dead tiles
   static constexpr int kTiles = 2 * kTile > kT ? 2 * kTile : kT;
-  static constexpr int kSmem = kTiles + 2 * kMat + (2 * 4 * kC + 2 * kC * 2 + 2 * kC + 8) * 4;
+  static constexpr int kSmem = kTiles + 2 * kMat + (2 * 4 * kC + 2 * kC * 3 + 2 * kC + 8) * 4;
 };
+
+// G_i - G_j of sums kept in two terms each: after strong decays both are large, and what
+// one fp32 term leaves of their difference (2^-10 at 9600) would reach the state.
+__device__ __forceinline__ float log_decay(float gi, float li, float gj, float lj) { return (gi - gj) + (li - lj); }
 
 // exp(G_i - G_j) and the norms times the products of 16-row block I with the keys: P (ROLE
 // 1), or I + A's strictly lower part and B_10 (ROLE 0). Left of the diagonal block the
 // exponential is one factor of the row's by one of the column's, both at most 1.
 template <int ROLE, int I>
-__device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int heads, uint8_t* rec0, const float* sG,
+__device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int heads, uint8_t* rec0, const float* sG, const float* sL,
                                               const float* sB, const float* sRk, const float* sRow, const float* sW,
                                               float* A, int quad, int t4) {
   const int i0 = 16 * I + quad;
 #pragma unroll 1
   for (int h = 0; h < heads; ++h) {
-    const float *hG = sG + h * kC, *hW = sW + (h * 4 + I) * kC + 2 * t4;
+    const float *hG = sG + h * kC, *hL = sL + h * kC, *hW = sW + (h * 4 + I) * kC + 2 * t4;
     uint8_t* to = rec0 + h * kRecBytes + (ROLE ? 2 * kRecT : 0) + (i0 * kC + 2 * t4) * 2;
     float* Ah = A + (h * kC + i0) * kLd + 2 * t4;
-    float g[2], f[2], a[2], b[2];
+    float f[2], a[2], b[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      g[half] = hG[i0 + 8 * half];
-      f[half] = sRow[i0 + 8 * half];
-      a[half] = I > 0 ? exp2_fast(g[half] - hG[I > 0 ? 16 * I - 1 : 0]) * f[half] : 0.f;
+      const int i = i0 + 8 * half, end = I > 0 ? 16 * I - 1 : 0;
+      f[half] = sRow[i];
+      a[half] = I > 0 ? exp2_fast(log_decay(hG[i], hL[i], hG[end], hL[end])) * f[half] : 0.f;
       b[half] = ROLE ? 1.f : sB[h * kC + i0 + 8 * half];
     }
 #pragma unroll
@@ -271,12 +275,14 @@ __device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int head
           e[half][1] = acc[n][2 * half + 1] * a[half] * w.y;
         }
       } else {  // nothing above the diagonal (there the difference may overflow)
-        const float2 gj = *reinterpret_cast<const float2*>(hG + j), rj = *reinterpret_cast<const float2*>(sRk + j);
+        const float2 gj = *reinterpret_cast<const float2*>(hG + j), lj = *reinterpret_cast<const float2*>(hL + j),
+                     rj = *reinterpret_cast<const float2*>(sRk + j);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int i = i0 + 8 * half;
-          e[half][0] = j <= i - (ROLE ? 0 : 1) ? exp2_fast(g[half] - gj.x) * (rj.x * f[half]) * acc[n][2 * half] : 0.f;
-          e[half][1] = j + 1 <= i - (ROLE ? 0 : 1) ? exp2_fast(g[half] - gj.y) * (rj.y * f[half]) * acc[n][2 * half + 1] : 0.f;
+          const float gi = hG[i], li = hL[i];
+          e[half][0] = j <= i - (ROLE ? 0 : 1) ? exp2_fast(log_decay(gi, li, gj.x, lj.x)) * (rj.x * f[half]) * acc[n][2 * half] : 0.f;
+          e[half][1] = j + 1 <= i - (ROLE ? 0 : 1) ? exp2_fast(log_decay(gi, li, gj.y, lj.y)) * (rj.y * f[half]) * acc[n][2 * half + 1] : 0.f;
         }
       }
 #pragma unroll
@@ -309,7 +315,8 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
   float* A = reinterpret_cast<float*>(smem + Sh::kTiles);        // [2][64][kLd]
   float* sW = A + 2 * kC * kLd;  // [2][4][64] exp(G at the end of block I - 1 minus G_j) / |k_j|, j before block I
   float* sG = sW + 2 * 4 * kC;   // [2][64] sums of g, in units of log2
-  float* sB = sG + 2 * kC;       // [2][64]
+  float* sL = sG + 2 * kC;       // [2][64] their second terms
+  float* sB = sL + 2 * kC;       // [2][64]
   float* sRk = sB + 2 * kC;
   float* sRq = sRk + kC;
   int* sSeq = reinterpret_cast<int*>(sRq + kC);  // [warps]
@@ -346,21 +353,24 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
     for (int x = 0; x < 2; ++x) {
       const int t = 2 * lane + x;
       const bool in = t < nt && hv0 + warp < (hk + 1) * d.rep;
-      // (a decay to below 2^-126 is 0 either way; the bound keeps later differences exact
-      // and takes g = -infinity, a reset)
+      // (a decay to below 2^-126 is 0 either way; the bound takes g = -infinity, a reset)
       g[x] = in ? __ldg(d.g + (t0 + t) * d.g_stride + hv0 + warp) * 1.4426950408889634f : 0.f;
       g[x] = g[x] < -150.f ? -150.f : g[x];
       be[x] = in ? __ldg(d.beta + (t0 + t) * d.beta_stride + hv0 + warp) : 0.f;
     }
-    float sum = g[0] + g[1];
+    double sum = static_cast<double>(g[0]) + g[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const float y = __shfl_up_sync(0xffffffffu, sum, o);
+      const double y = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += y;
     }
-    float before = __shfl_up_sync(0xffffffffu, sum, 1);
-    if (lane == 0) before = 0.f;
-    *reinterpret_cast<float2*>(sG + warp * kC + 2 * lane) = make_float2(before + g[0], sum);
+    double before = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane == 0) before = 0.0;
+    before += g[0];
+    const float2 hi = make_float2(static_cast<float>(before), static_cast<float>(sum));
+    *reinterpret_cast<float2*>(sG + warp * kC + 2 * lane) = hi;
+    *reinterpret_cast<float2*>(sL + warp * kC + 2 * lane) =
+        make_float2(static_cast<float>(before - hi.x), static_cast<float>(sum - hi.y));
     *reinterpret_cast<float2*>(sB + warp * kC + 2 * lane) = make_float2(be[0], be[1]);
   };
   gates(hk * d.rep);  // while the tiles are on their way
@@ -410,26 +420,30 @@ __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const
     if (gh < heads) {
       float* f = reinterpret_cast<float*>(rec0 + gh * kRecBytes + kRecScal);
       const float G = sG[gh * kC + gt], end = sG[gh * kC + kC - 1];
+      const float after = log_decay(end, sL[gh * kC + kC - 1], G, sL[gh * kC + gt]);
       f[gt] = exp2_fast(G) * sRk[gt];
       f[kC + gt] = exp2_fast(G) * sRq[gt];
-      f[2 * kC + gt] = exp2_fast(end - G) * sRk[gt];
+      f[2 * kC + gt] = exp2_fast(after) * sRk[gt];
       if (gt == 0) f[3 * kC] = exp2_fast(end);
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int x = e * kPrepThreads + tid, h = x >> 8, block = (x >> 6) & 3, j = x & (kC - 1);
-      if (j < 16 * block) sW[x] = exp2_fast(sG[h * kC + 16 * block - 1] - sG[h * kC + j]) * sRk[j];
+      if (j < 16 * block) {
+        const int at = h * kC + 16 * block - 1;
+        sW[x] = exp2_fast(log_decay(sG[at], sL[at], sG[h * kC + j], sL[h * kC + j])) * sRk[j];
+      }
     }
     __syncthreads();
     switch (warp) {  // each with its own straight code: shared and predicated it took twice as long
-      case 0: prep_elements<0, 0>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
-      case 1: prep_elements<0, 1>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
-      case 2: prep_elements<0, 2>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
-      case 3: prep_elements<0, 3>(acc, heads, rec0, sG, sB, sRk, sRk, sW, A, quad, t4); break;
-      case 4: prep_elements<1, 0>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
-      case 5: prep_elements<1, 1>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
-      case 6: prep_elements<1, 2>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
-      default: prep_elements<1, 3>(acc, heads, rec0, sG, sB, sRk, sRq, sW, A, quad, t4); break;
+      case 0: prep_elements<0, 0>(acc, heads, rec0, sG, sL, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 1: prep_elements<0, 1>(acc, heads, rec0, sG, sL, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 2: prep_elements<0, 2>(acc, heads, rec0, sG, sL, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 3: prep_elements<0, 3>(acc, heads, rec0, sG, sL, sB, sRk, sRk, sW, A, quad, t4); break;
+      case 4: prep_elements<1, 0>(acc, heads, rec0, sG, sL, sB, sRk, sRq, sW, A, quad, t4); break;
+      case 5: prep_elements<1, 1>(acc, heads, rec0, sG, sL, sB, sRk, sRq, sW, A, quad, t4); break;
+      case 6: prep_elements<1, 2>(acc, heads, rec0, sG, sL, sB, sRk, sRq, sW, A, quad, t4); break;
+      default: prep_elements<1, 3>(acc, heads, rec0, sG, sL, sB, sRk, sRq, sW, A, quad, t4); break;
     }
     __syncthreads();
     // (I + A)^-1 of the diagonal blocks of 16, one per warp: columns of the two blocks of
