@@ -547,6 +547,65 @@ struct WalkShape {
   static_assert(kSmem <= (PAIR ? 227 : 113) * 1024);
 };
 
+// Tokens from t0 on one after another, as the rule is defined, for the 16 value columns from
+// `col` of value head hv: one warp, s laid out as in the walk. Ends at t1, or when the state's
+// columns quad (lost0) and quad + 8 (lost1) that were asked for are not finite any more.
+template <int DK>
+__device__ __noinline__ void delta_tokens(float (&s)[DK / 8][4], const DeltaArgs d, int t0, int t1, int hv, int dv, int col,
+                                          bool lost0, bool lost1) {
+  const int lane = threadIdx.x & 31, quad = lane >> 2, t4 = lane & 3, hk = hv / d.rep;
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(d.k + t * d.k_stride + hk * DK) + t4;
+    const uint32_t* qp = reinterpret_cast<const uint32_t*>(d.q + t * d.q_stride + hk * DK) + t4;
+    const __nv_bfloat16* vp = d.v + t * d.v_stride + hv * dv + col + quad;
+    const float eg = expf(__ldg(d.g + t * d.g_stride + hv)), beta = __ldg(d.beta + t * d.beta_stride + hv);
+    float kk = 0.f, qq = 0.f, x[2] = {}, y[2] = {};
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n) {
+      const uint32_t w = __ldg(kp + 4 * n);
+      const float k0 = __uint_as_float(w << 16), k1 = __uint_as_float(w & 0xffff0000u);
+      kk = fmaf(k0, k0, fmaf(k1, k1, kk));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        s[n][2 * c] *= eg;
+        s[n][2 * c + 1] *= eg;
+        x[c] = fmaf(s[n][2 * c], k0, fmaf(s[n][2 * c + 1], k1, x[c]));
+      }
+    }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {  // the 4 lanes of a column
+      kk += __shfl_xor_sync(0xffffffffu, kk, o);
+      x[0] += __shfl_xor_sync(0xffffffffu, x[0], o);
+      x[1] += __shfl_xor_sync(0xffffffffu, x[1], o);
+    }
+    const float rk = d.l2norm ? rsqrtf(kk + d.eps) : 1.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) x[c] = beta * (__bfloat162float(vp[8 * c]) - rk * x[c]) * rk;
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n) {
+      const uint32_t w = __ldg(kp + 4 * n), z = __ldg(qp + 4 * n);
+      const float q0 = __uint_as_float(z << 16), q1 = __uint_as_float(z & 0xffff0000u);
+      qq = fmaf(q0, q0, fmaf(q1, q1, qq));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        s[n][2 * c] = fmaf(__uint_as_float(w << 16), x[c], s[n][2 * c]);
+        s[n][2 * c + 1] = fmaf(__uint_as_float(w & 0xffff0000u), x[c], s[n][2 * c + 1]);
+        y[c] = fmaf(s[n][2 * c], q0, fmaf(s[n][2 * c + 1], q1, y[c]));
+      }
+    }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      qq += __shfl_xor_sync(0xffffffffu, qq, o);
+      y[0] += __shfl_xor_sync(0xffffffffu, y[0], o);
+      y[1] += __shfl_xor_sync(0xffffffffu, y[1], o);
+    }
+    const float rq = d.scale * (d.l2norm ? rsqrtf(qq + d.eps) : 1.f);
+    if (t4 < 2) d.out[t * d.out_stride + hv * dv + col + quad + 8 * t4] = __float2bfloat16_rn(rq * (t4 ? y[1] : y[0]));
+    if (!__any_sync(0xffffffffu, (lost0 && isfinite(s[0][0])) || (lost1 && isfinite(s[0][2])))) return;
+  }
+}
+
 // One CTA per (16 W value columns, value head, sequence) walks the sequence's
 // chunks. Warp w holds the transposed state of its 16 value columns, [16, DK], as
 // mma accumulators: these are laid out like A operands, so the state, R and N go from
@@ -858,6 +917,22 @@ __global__ void __launch_bounds__(32 * W * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_d
 #pragma unroll
         for (int y = 0; y < 4; ++y) s[n + x][y] = fmaf(s[n + x][y], end, p[x][y]);
     }
+  }
+  // What is not finite meets the zeros above the diagonals of T and P and so reaches tokens up
+  // to 15 before its own. It also stays in its columns of the state for good, every row of
+  // them, so one look at the end finds it (asked in each chunk it cost 6 of 94 us); the warp then
+  // writes its outputs up to there once more, token by token (1.7 us each). Later ones and the
+  // state are as they should be.
+  if (PAIR) __syncthreads();  // the second warps' outputs are written
+  const bool lost0 = !second && !isfinite(s[0][0]), lost1 = !second && !isfinite(s[0][2]);
+  if (__any_sync(0xffffffffu, lost0 || lost1) && c0 < c1) {
+    float x[DK / 8][4];
+#pragma unroll
+    for (int n = 0; n < DK / 8; ++n)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[n][y] = zero ? 0.f : S[(n * 8 + 2 * t4 + (y & 1)) * DV + quad + (y >> 1) * 8];
+    __syncwarp();  // other lanes' outputs of the same columns
+    delta_tokens<DK>(x, d, c0, c1, hv, DV, col + 16 * warp, lost0, lost1);
   }
 #pragma unroll
   for (int n = 0; n < DK / 8; ++n)

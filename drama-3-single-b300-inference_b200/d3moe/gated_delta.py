@@ -53,7 +53,8 @@ def gated_delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     """Packed prompts: rows [cu_seqlens[i], cu_seqlens[i+1]) (int32 [n+1]) are
     sequence i's tokens. Each sequence starts from state[slots[i]] (None:
     state[i]), or from zero where fresh[i] (bool [n]), and leaves its state
-    there. Other arguments and the result are those of gated_delta_step. The
-    lengths are read on the device, so the call can be captured."""
+    there. Other arguments and the result are those of gated_delta_step; out must
+    not overlap q, k or v. The lengths are read on the device, so the call can be
+    captured."""
     return _native.gated_delta_chunk(q, k, v, g, beta, state, cu_seqlens, slots, fresh, scale, l2norm, eps, out,
                                      workspace, status)

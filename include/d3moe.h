@@ -551,7 +551,8 @@ D3_API int d3_gated_delta_step(const d3_gated_delta_t* args, int n, int32_t* sta
  * <= T; rows that belong to no sequence are not written). fresh (uint8 [n], may
  * be NULL): a sequence whose entry is not 0 starts from a zero state instead of
  * its slot's. A sequence without tokens leaves its state as it is, or zeroes it
- * when fresh. */
+ * when fresh. out must not overlap q, k or v. What is not finite in a token's
+ * operands reaches that token and later ones only. */
 D3_API int d3_gated_delta_chunk_workspace_size(int T, int n, int value_heads, int key_dim,
                                                int value_dim, size_t* bytes);
 D3_API int d3_gated_delta_chunk(const d3_gated_delta_t* args, const int32_t* cu, int T, int n,
