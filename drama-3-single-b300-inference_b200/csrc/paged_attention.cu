@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kAttnThreads, (AttnShape<DT, D, WIDE>::kCtas))
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           int e = 0;
           if (top > 0.f && isfinite(top)) frexpf(top, &e);
-          e = max(-100, min(100, e));  // 2^-e and 2^e both exist
+          e = max(-126, min(126, e));  // 2^-e and 2^e both exist (the largest bf16 becomes 4)
           const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
           // k index 2 t4 + {0, 1, 8, 9} stands for column 4 t4 + {0, 1, 2, 3}, as in the keys below
 #pragma unroll

@@ -63,3 +63,16 @@ def test_small_probabilities_beside_a_large_one(dtype, gap, lens, q_heads, heads
     assert (excess <= 0).all(), f"{float(((got.double() - want).abs() / want.abs().clamp(min=1e-30)).max())} of the result"
     live = ~torch.isinf(wlse)
     assert ((lse.double() - wlse).abs()[live] <= bl[live]).all()
+
+
+@pytest.mark.parametrize("power", [-120, -60, 60, 122])
+def test_queries_of_any_power_of_two_over_an_e4m3_cache(power):
+    """Queries times 2^p with a scale of 2^-p are the same operands: no bit changes."""
+    from d3moe import attention
+    k, v, table, _, _ = make_cache([90, 40], 2, 64, 16, FP8)
+    q = torch.randn((2, 8, 64), generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    ln = torch.tensor([90, 40], dtype=torch.int32, device="cuda")
+    q = torch.where(q.abs() < 2.0 ** -5, torch.zeros_like(q), q)  # the others stay normal numbers
+    want = attention.paged_attention(q, k, v, table, ln, 2.0 ** -3)
+    got = attention.paged_attention((q.float() * 2.0 ** power).to(BF16), k, v, table, ln, 2.0 ** (-3 - power))
+    assert torch.isfinite(want).all() and torch.equal(got, want)
