@@ -72,12 +72,6 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
-template <bool BF16>
-__device__ __forceinline__ float unpack16(uint16_t b) {
-  if constexpr (BF16) return bf16_bits_to_f32(b);
-  return __half2float(__ushort_as_half(b));
-}
-
 // Byte offset of 16-byte piece c of row r of a shared-memory tile: pieces are permuted so
 // that the 8 rows of an ldmatrix tile fall into different banks.
 template <int ROW_BYTES>

@@ -40,7 +40,7 @@
 //
 // An e4m3 cache is widened to f16 in registers (exact). Its queries are scaled by
 // a power of two per row into f16's range (exact for every element within 2^-14
-// of the row's largest, error below 2^-25 of that otherwise).
+// of the row's largest, error at most 2^-24 of that otherwise).
 #include "kv_cache.cuh"
 #include "mma_tiles.cuh"
 
