@@ -891,6 +891,9 @@ extern "C" int d3_paged_attention(const void* q, int64_t q_row_stride, int64_t q
   D3_REQUIRE(q_dtype == (cache->dtype == D3_DTYPE_E4M3 ? D3_DTYPE_BF16 : cache->dtype),
              "queries of dtype %d for a cache of dtype %d", q_dtype, cache->dtype);
   D3_REQUIRE(max_len >= 0 && window >= 0, "negative length bound or window");
+  // an offset below zero marks a row past its sequence's end
+  D3_REQUIRE(cache->k_page_stride >= 0 && cache->k_token_stride >= 0 && cache->v_page_stride >= 0 && cache->v_token_stride >= 0,
+             "negative page or token stride");
   D3_REQUIRE(cache->sequences == B, "the page table must have one row per query");
   if (workspace_bytes < need || !workspace)
     return set_error(D3_EWORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -500,6 +500,7 @@ D3_API int d3_copy_pages(void* pool, int planes, int64_t plane_stride, int pages
  * length 0 gives a zero row and lse = -infinity. lens int32 [B]; max_len is
  * the host's bound on lens (a longer sequence is read up to max_len, and none
  * past the table). dim 64, 128 or 256; q_heads a multiple of the cache's heads.
+ * Page and token strides of the cache must not be negative here.
  * Logits, softmax statistics and sums are fp32. Replaces the reference's paged
  * decode (src/drama3/model.py:55-141). */
 D3_API int d3_paged_attention_workspace_size(int B, int q_heads, int kv_heads, int dim,
