@@ -1066,6 +1066,7 @@ extern "C" int d3_gated_delta_chunk(const d3_gated_delta_t* args, const int32_t*
                                     int32_t* status, d3_stream_t stream) {
   DeltaArgs a{};
   if (int rc = delta_args(args, n, T, status, a)) return rc;
+  D3_REQUIRE(T <= 0x7fffff00, "too many tokens for one call");  // the last chunk's counter passes T
   size_t need = 0;
   if (int rc = d3_gated_delta_chunk_workspace_size(T, n, args->value_heads, args->key_dim, args->value_dim, &need)) return rc;
   if (workspace_bytes < need || (need && !workspace))
