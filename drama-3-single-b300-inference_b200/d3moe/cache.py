@@ -40,7 +40,8 @@ class PagedCache:
 
       seq = cache.new()          an empty sequence
       cache.extend(seq, n)       room for n more tokens (write them with kv_append)
-      child = cache.fork(seq)    shares the full pages; a part-filled last page is copied
+      child = cache.fork(seq)    shares the full pages; a part-filled last page is copied (tokens that
+                                 have room but are not written yet: see fork)
       cache.free(seq)            gives back the pages no other sequence holds
       cache.compact()            moves the pages in use to the lowest numbers
     """
@@ -113,15 +114,23 @@ class PagedCache:
         self._write_row(seq, first)
         return range(n, n + tokens)
 
-    def fork(self, seq: int) -> int:
+    def fork(self, seq: int, written: int | None = None) -> int:
         """A new sequence with the same tokens. No page that either may still write
-        is shared: a part-filled last page gets its copy here."""
+        is shared: a part-filled last page gets its copy here. `written`: how many of
+        the sequence's tokens have been written (on the current stream) so far; by
+        default all that extend made room for. Pages that hold others are the child's
+        own, so each of the two writes its own tokens from there on."""
         self._alive(seq)
-        full = self.lens[seq] // self.page_size
-        part = self._pages[seq][full:]
+        if written is None:
+            written = self.lens[seq]
+        if not 0 <= written <= self.lens[seq]:
+            raise ValueError(f"sequence {seq} has {self.lens[seq]} tokens, {written} cannot have been written")
+        full = written // self.page_size
+        rest = self._pages[seq][full:]  # the first of them may be part-filled, the others are not written yet
+        part = rest[:written % self.page_size > 0]
         child = self.new()
         try:
-            copies = self._take(len(part))
+            copies = self._take(len(rest))
         except RuntimeError:
             self.lens[child] = None
             raise
@@ -131,7 +140,7 @@ class PagedCache:
         self._pages[child] = shared + copies
         self.lens[child] = self.lens[seq]
         if part:
-            self._copy(part, copies)
+            self._copy(part, copies[:1])
         self._write_row(child)
         return child
 

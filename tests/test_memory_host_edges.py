@@ -34,3 +34,45 @@ def test_delta_chunk_refuses_tokens_whose_counter_would_pass_32_bits():
     a = _lib.D3GatedDelta(q=4096, k=4096, v=4096, g=4096, beta=4096, out=4096, state=4096, slots=1, key_heads=1, value_heads=1, key_dim=64,
                           value_dim=64, l2norm=1, scale=1.0, eps=1e-6)
     _refused(lib.d3_gated_delta_chunk(ctypes.byref(a), 4096, 2**31 - 1, 1, None, 4096, 1 << 60, None, None), b"too many tokens")
+
+
+@pytest.mark.parametrize("room,written", [(10, 0), (10, 3), (10, 4), (10, 7), (10, 8), (10, 10), (3, 0), (8, 8), (0, 0)])
+def test_a_fork_shares_no_page_that_is_still_to_be_written(room, written):
+    """A fork between extend and the writes: parent and child then write tokens of their own."""
+    from test_memory_host import HostCache
+    c = HostCache(2, 16, 4, 1, 2, max_sequences=4, max_len=16)
+
+    def put(seq, t, x):
+        c.pool[:, :, int(c.table[seq, t // 4]), t % 4] = x
+
+    def held(seq):
+        return [float(c.pool[0, 0, int(c.table[seq, t // 4]), t % 4, 0, 0]) for t in range(c.lens[seq])]
+
+    a = c.new()
+    c.extend(a, room)
+    for t in range(written):
+        put(a, t, 1 + t)
+    b = c.fork(a, written)
+    for t in range(written, room):
+        put(a, t, 100 + t)
+        put(b, t, 200 + t)
+    for seq, base in ((a, 100), (b, 200)):
+        for t in c.extend(seq, 2):
+            put(seq, t, base + t)
+        assert held(seq) == [1 + t for t in range(written)] + [base + t for t in range(written, room + 2)]
+    shared = set(c._pages[a]) & set(c._pages[b])
+    assert len(shared) == written // 4 and sum(n > 0 for n in c._holders) == 2 * -(-(room + 2) // 4) - len(shared)
+    c.free(a)
+    c.free(b)
+    assert c.free_pages == 16
+
+
+def test_fork_refuses_more_written_tokens_than_there_are():
+    from test_memory_host import HostCache
+    c = HostCache(1, 8, 4, 1, 2, max_sequences=2, max_len=16)
+    a = c.new()
+    c.extend(a, 5)
+    for n in (6, -1):
+        with pytest.raises(ValueError, match="cannot have been written"):
+            c.fork(a, n)
+    assert c.lens[1] is None and c.free_pages == 6
