@@ -283,7 +283,8 @@ _NATIVE_CALLS = ("d3_kv_append", "d3_copy_pages", "d3_paged_attention", "d3_page
 
 def native():
     """The CPython binding (csrc/binding/), connected to the loaded library:
-    the operators a decode step calls many times reach the C ABI through it."""
+    the operators a decode step calls many times reach the C ABI through it. It is
+    loaded at their first call; the other operators do not need it."""
     global _native
     if _native is None:
         import importlib.machinery

@@ -20,8 +20,6 @@ import torch
 from . import _lib
 from ._lib import call
 
-_native = _lib.native()
-
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               page_table: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None = None, *,
@@ -32,7 +30,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     negative ones are skipped. An e4m3 cache takes bf16 rows and holds
     e4m3(clamp(x / scale[head], -448, 448)). Tokens past the table or on a page
     outside the cache are not written and set status to D3_STATUS_BAD_ROW."""
-    _native.kv_append(k, v, k_cache, v_cache, page_table, positions, seq_ids, k_scale, v_scale, status)
+    _lib.native().kv_append(k, v, k_cache, v_cache, page_table, positions, seq_ids, k_scale, v_scale, status)
 
 
 def paged_attention_workspace(batch: int, heads: int, kv_heads: int, dim: int, device) -> torch.Tensor:
@@ -53,5 +51,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (default: what the page table can hold). Returns out (q's dtype), or (out,
     lse f32 [B, heads]) with return_lse. An empty sequence gives zeros and
     lse = -inf. Nothing is read on the host, so the call can be captured."""
-    return _native.paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, window,
-                                   max_seq_len, out, return_lse, workspace, status)
+    return _lib.native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, window,
+                                         max_seq_len, out, return_lse, workspace, status)

@@ -17,8 +17,6 @@ import torch
 
 from . import _lib
 
-_native = _lib.native()
-
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_dim: int = 0, *,
                status: torch.Tensor | None = None) -> None:
@@ -28,7 +26,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, page_di
     and k / v). src and dst int32 [n] on the device; a negative number skips its
     pair, one past the pool too, with status set to D3_STATUS_BAD_ROW. No page
     may be both copied from and copied to in one call, nor copied to twice."""
-    _native.copy_pages(pool, src, dst, page_dim, status)
+    _lib.native().copy_pages(pool, src, dst, page_dim, status)
 
 
 class PagedCache:

@@ -19,8 +19,6 @@ import torch
 from . import _lib
 from ._lib import call
 
-_native = _lib.native()
-
 
 def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                      state: torch.Tensor, slots: torch.Tensor | None = None, *, scale: float | None = None,
@@ -32,7 +30,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     updated in place; a negative slot leaves the sequence out (zero row). q and
     k are divided by sqrt(|x|^2 + eps) when l2norm; scale: key_dim**-0.5 by
     default. Returns out bf16 [n, value_heads, value_dim]."""
-    return _native.gated_delta_step(q, k, v, g, beta, state, slots, scale, l2norm, eps, out, status)
+    return _lib.native().gated_delta_step(q, k, v, g, beta, state, slots, scale, l2norm, eps, out, status)
 
 
 def gated_delta_chunk_workspace(tokens: int, sequences: int, value_heads: int, key_dim: int, value_dim: int,
@@ -56,5 +54,5 @@ def gated_delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     there. Other arguments and the result are those of gated_delta_step; out must
     not overlap q, k or v. The lengths are read on the device, so the call can be
     captured."""
-    return _native.gated_delta_chunk(q, k, v, g, beta, state, cu_seqlens, slots, fresh, scale, l2norm, eps, out,
-                                     workspace, status)
+    return _lib.native().gated_delta_chunk(q, k, v, g, beta, state, cu_seqlens, slots, fresh, scale, l2norm, eps, out,
+                                           workspace, status)

@@ -76,3 +76,31 @@ def test_fork_refuses_more_written_tokens_than_there_are():
         with pytest.raises(ValueError, match="cannot have been written"):
             c.fork(a, n)
     assert c.lens[1] is None and c.free_pages == 6
+
+
+def test_the_package_imports_without_the_binding():
+    """Only a call of a sequence-memory operator needs _d3native.so; the others reach libd3moe.so by ctypes."""
+    import subprocess
+    import sys
+
+    from conftest import PKG_DIR
+    code = """
+from d3moe import _lib
+def missing():
+    raise ImportError("no binding here")
+_lib.native = missing
+import torch
+from d3moe import attention, cache, gated_delta, torch_ops
+torch.ops.d3moe.moe_layer, torch.ops.d3moe.paged_attention
+t = torch.zeros(1)
+for f, a in ((attention.kv_append, (t,) * 6), (attention.paged_attention, (t,) * 5), (cache.copy_pages, (t,) * 3),
+             (gated_delta.gated_delta_step, (t,) * 6), (gated_delta.gated_delta_chunk, (t,) * 7)):
+    try:
+        f(*a)
+    except ImportError as e:
+        assert "no binding here" in str(e)
+    else:
+        raise AssertionError(f)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=PKG_DIR, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
