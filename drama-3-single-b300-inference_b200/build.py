@@ -3,7 +3,9 @@ CPython binding _d3native.so (csrc/binding/) with g++.
 
 The libraries are written in-tree next to the Python package (d3moe/_lib/) so
 that they travel with the source tree; they are rebuilt only when a source or
-header is newer than they are.
+header is newer than they are, the binding also when the installed torch is not
+the one it was built for. Without torch libd3moe.so is built alone: it needs
+nvcc only, the binding g++ and torch as well.
 
 Usage: python build.py [--force] [--verbose]
 """
@@ -51,13 +53,42 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
-def needs_build() -> bool:
-    built = (LIB, SELFTEST_LIB, NATIVE_LIB)
+def torch_version() -> str | None:
+    """Version of the installed torch (without importing it), None when there is none."""
+    import importlib.metadata
+
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+def binding_mark(version: str | None) -> str:
+    """The text by which the binding says which torch it was built for."""
+    return f"d3moe binding for torch {version};"
+
+
+def _older(built: tuple[Path, ...], sources: list[Path]) -> bool:
     if not all(p.exists() for p in built):
         return True
     lib_time = min(p.stat().st_mtime for p in built)
-    deps = list(CSRC.rglob("*")) + list(INCLUDE.glob("*.h")) + [Path(__file__)]
+    deps = sources + list(INCLUDE.glob("*.h")) + [Path(__file__)]
     return any(p.stat().st_mtime > lib_time for p in deps if p.is_file())
+
+
+def library_needs_build() -> bool:
+    return _older((LIB, SELFTEST_LIB), [p for p in CSRC.rglob("*") if p.parent.name != "binding"])
+
+
+def binding_needs_build() -> bool:
+    version = torch_version()
+    if version is None:
+        return False
+    return _older((NATIVE_LIB,), list((CSRC / "binding").glob("*"))) or binding_mark(version).encode() not in NATIVE_LIB.read_bytes()
+
+
+def needs_build() -> bool:
+    return library_needs_build() or binding_needs_build()
 
 
 def _link(cc: str, srcs: list[Path], out: Path, objdir: Path, verbose: bool) -> None:
@@ -91,6 +122,7 @@ def _link_binding(out: Path, verbose: bool) -> None:
                cuda / "include", Path(sysconfig.get_paths()["include"])]
     tmp = out.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f'-DD3_BUILT_FOR="{binding_mark(torch_version())}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *[f"-I{p}" for p in include], *map(str, sorted((CSRC / "binding").glob("*.cpp"))), "-o", str(tmp),
            f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
@@ -101,15 +133,18 @@ def _link_binding(out: Path, verbose: bool) -> None:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not needs_build():
-        return LIB
+    library = force or library_needs_build()
     OUT_DIR.mkdir(parents=True, exist_ok=True)
     objdir = HERE / "_build"
     objdir.mkdir(exist_ok=True)
-    cc = nvcc()
-    _link(cc, sources(), LIB, objdir, verbose)
-    _link(cc, sorted((CSRC / "selftest").glob("*.cu")), SELFTEST_LIB, objdir, verbose)
-    _link_binding(NATIVE_LIB, verbose)
+    if library:
+        cc = nvcc()
+        _link(cc, sources(), LIB, objdir, verbose)
+        _link(cc, sorted((CSRC / "selftest").glob("*.cu")), SELFTEST_LIB, objdir, verbose)
+    if torch_version() is None:
+        print("torch is not installed: the CPython binding of the sequence-memory operators is left out", file=sys.stderr)
+    elif force or binding_needs_build():
+        _link_binding(NATIVE_LIB, verbose)
     return LIB
 
 

@@ -434,4 +434,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_d3native", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__d3native() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__d3native() {
+  PyObject* m = PyModule_Create(&module);
+  // the text is also what build.py looks for in the file
+  if (m && PyModule_AddStringConstant(m, "built_for", D3_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -104,3 +104,63 @@ for f, a in ((attention.kv_append, (t,) * 6), (attention.paged_attention, (t,) *
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=PKG_DIR, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.fixture
+def builder(tmp_path, monkeypatch):
+    """build.py with its outputs in a folder of their own, and a record of what it would link."""
+    import importlib.util
+
+    from conftest import PKG_DIR
+    spec = importlib.util.spec_from_file_location("d3moe_build_edges", PKG_DIR / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    for name in ("LIB", "SELFTEST_LIB", "NATIVE_LIB"):
+        monkeypatch.setattr(b, name, tmp_path / getattr(b, name).name)
+    monkeypatch.setattr(b, "OUT_DIR", tmp_path)
+    monkeypatch.setattr(b, "HERE", tmp_path)
+    b.linked = []
+
+    def link(cc, srcs, out, objdir, verbose):
+        b.linked.append(out.name)
+        out.write_bytes(b"")
+
+    def binding(out, verbose):
+        b.linked.append(out.name)
+        out.write_bytes(f"...{b.binding_mark(b.torch_version())}...".encode())
+
+    monkeypatch.setattr(b, "_link", link)
+    monkeypatch.setattr(b, "_link_binding", binding)
+    monkeypatch.setattr(b, "nvcc", lambda: "nvcc")
+    return b
+
+
+def test_the_binding_is_rebuilt_for_another_torch(builder, monkeypatch):
+    monkeypatch.setattr(builder, "torch_version", lambda: "2.0+x")
+    builder.build()
+    assert builder.linked == ["libd3moe.so", "libd3moe_selftest.so", "_d3native.so"] and not builder.needs_build()
+    monkeypatch.setattr(builder, "torch_version", lambda: "2.0")
+    assert builder.needs_build()
+    builder.linked.clear()
+    builder.build()
+    assert builder.linked == ["_d3native.so"] and not builder.needs_build()
+
+
+def test_without_torch_the_library_is_built_alone(builder, monkeypatch, capsys):
+    monkeypatch.setattr(builder, "torch_version", lambda: None)
+    builder.build()
+    assert builder.linked == ["libd3moe.so", "libd3moe_selftest.so"] and not builder.needs_build()
+    assert "binding" in capsys.readouterr().err
+    monkeypatch.setattr(builder, "torch_version", lambda: "2.0")  # torch came later
+    assert builder.needs_build()
+
+
+def test_the_binding_in_the_tree_names_the_torch_it_is_for():
+    import importlib.util
+
+    from conftest import PKG_DIR
+    from d3moe import _lib
+    spec = importlib.util.spec_from_file_location("d3moe_build_mark", PKG_DIR / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    assert _lib.native().built_for == b.binding_mark(b.torch_version())
