@@ -237,15 +237,16 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t axis = integer(p[3], "page_dim");
     require(axis >= 0 && axis < pool.dim(), "page_dim must be an axis of pool");
     const IntArrayRef size = pool.sizes(), stride = pool.strides();
+    const bool none = pool.numel() == 0;  // nothing to copy: no stride of it means anything
     int64_t elements = 1, planes = 1, plane_stride = 0;
     for (int64_t i = pool.dim() - 1; i > axis; --i) {
-      require(size[i] == 1 || stride[i] == elements, "the axes behind page_dim must be contiguous");
+      require(none || size[i] == 1 || stride[i] == elements, "the axes behind page_dim must be contiguous");
       elements *= size[i];
     }
     for (int64_t i = axis - 1; i >= 0; --i) {
       if (size[i] == 1) continue;
       if (planes == 1) plane_stride = stride[i];
-      else require(stride[i] == planes * plane_stride, "the axes before page_dim must step evenly");
+      else require(none || stride[i] == planes * plane_stride, "the axes before page_dim must step evenly");
       planes *= size[i];
     }
     const Tensor& src = tensor(p[1], "src");
@@ -254,6 +255,7 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t* dp = index_ptr(tensor(p[2], "dst"), count, dev, "dst");
     int32_t* status = status_ptr(p[4], dev);
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    if (none) Py_RETURN_NONE;
     check(copy_pages_fn(pool.data_ptr(), to_int(planes), plane_stride * b, to_int(size[axis]), stride[axis] * b, elements * b, sp, dp,
                         to_int(count), status, stream_of(dev)),
           "d3_copy_pages");
