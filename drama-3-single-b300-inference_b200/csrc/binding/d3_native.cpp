@@ -122,6 +122,9 @@ const float* scale_ptr(PyObject* o, int64_t heads, int dev) {
   return static_cast<const float*>(t->data_ptr());
 }
 
+// Stride of an axis; 0 where the axis has one entry and its stride no meaning.
+int64_t step(const Tensor& t, int axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
+
 d3_stream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 
 Tensor empty(IntArrayRef sizes, at::ScalarType type, int dev) {
@@ -153,21 +156,21 @@ d3_kv_cache_t kv_cache(const Tensor& k, const Tensor& v, const Tensor& table, Py
   const int dtype = dtype_tag(k.scalar_type());
   require(dtype >= 0 && v.scalar_type() == k.scalar_type(), "k_cache and v_cache must both be bfloat16, float16 or float8_e4m3fn");
   require(k.dim() == 4 && k.sizes() == v.sizes(), "k_cache and v_cache must be [pages, page_size, heads, dim] of one shape");
-  const IntArrayRef n = k.sizes(), ks = k.strides(), vs = v.strides();
-  require(ks[3] == 1 && vs[3] == 1, "the last axis of a cache must be contiguous");
-  require(table.scalar_type() == at::kInt && table.dim() == 2 && table.stride(1) == 1,
+  const IntArrayRef n = k.sizes();
+  require(k.stride(3) == 1 && v.stride(3) == 1, "the last axis of a cache must be contiguous");
+  require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1),
           "page_table must be int32 [sequences, pages per sequence], rows contiguous");
   require(on(v, dev) && on(table, dev), "caches and page_table must be on one device");
   require(dtype == D3_DTYPE_E4M3 || (k_scale == Py_None && v_scale == Py_None), "only an e4m3 cache has scales");
   d3_kv_cache_t c{};
   c.k = k.data_ptr();
   c.v = v.data_ptr();
-  c.k_page_stride = ks[0];
-  c.k_token_stride = ks[1];
-  c.k_head_stride = ks[2];
-  c.v_page_stride = vs[0];
-  c.v_token_stride = vs[1];
-  c.v_head_stride = vs[2];
+  c.k_page_stride = step(k, 0);
+  c.k_token_stride = step(k, 1);
+  c.k_head_stride = step(k, 2);
+  c.v_page_stride = step(v, 0);
+  c.v_token_stride = step(v, 1);
+  c.v_head_stride = step(v, 2);
   c.k_scale = scale_ptr(k_scale, n[2], dev);
   c.v_scale = scale_ptr(v_scale, n[2], dev);
   c.table = static_cast<const int32_t*>(table.data_ptr());
@@ -222,7 +225,7 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int32_t* sp = seq ? index_ptr(*seq, T, dev, "seq_ids") : nullptr;
     int32_t* status = status_ptr(p[9], dev);
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
-    check(kv_append_fn(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), dtype_tag(want), to_int(T),
+    check(kv_append_fn(k.data_ptr(), step(k, 0), step(k, 1), v.data_ptr(), step(v, 0), step(v, 1), dtype_tag(want), to_int(T),
                        sp, pos, &c, status, stream_of(dev)),
           "d3_kv_append");
     Py_RETURN_NONE;
@@ -296,8 +299,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     size_t need = 0, bytes = 0;
     check(paged_attention_ws_fn(to_int(B), to_int(Hq), c.heads, c.dim, &need), "d3_paged_attention_workspace_size");
     void* ws = scratch(p[12], need, dev, hold, bytes);
-    check(paged_attention_fn(q.data_ptr(), q.stride(0), q.stride(1), dtype_tag(want), to_int(B), to_int(Hq), &c, lens, to_int(limit),
-                             window, static_cast<float>(scale), out.data_ptr(), out.stride(0), out.stride(1),
+    check(paged_attention_fn(q.data_ptr(), step(q, 0), step(q, 1), dtype_tag(want), to_int(B), to_int(Hq), &c, lens, to_int(limit),
+                             window, static_cast<float>(scale), out.data_ptr(), step(out, 0), step(out, 1),
                              with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, ws, bytes, status, stream_of(dev)),
           "d3_paged_attention");
     if (!with_lse) return THPVariable_Wrap(out);
@@ -355,13 +358,13 @@ Delta delta(PyObject* const* p, PyObject* slots, int64_t n, PyObject* scale, PyO
   a.beta = static_cast<const float*>(beta.data_ptr());
   a.out = d.out.data_ptr();
   a.state = static_cast<float*>(state.data_ptr());
-  a.q_stride = q.stride(0);
-  a.k_stride = k.stride(0);
-  a.v_stride = v.stride(0);
-  a.g_stride = g.stride(0);
-  a.beta_stride = beta.stride(0);
-  a.out_stride = d.out.stride(0);
-  a.slot_stride = state.stride(0);
+  a.q_stride = step(q, 0);
+  a.k_stride = step(k, 0);
+  a.v_stride = step(v, 0);
+  a.g_stride = step(g, 0);
+  a.beta_stride = step(beta, 0);
+  a.out_stride = step(d.out, 0);
+  a.slot_stride = step(state, 0);
   a.slots = to_int(state.size(0));
   a.key_heads = to_int(Hk);
   a.value_heads = to_int(Hv);
