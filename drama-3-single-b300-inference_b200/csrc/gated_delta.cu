@@ -33,17 +33,19 @@
 // itself (together 2e-6 to 5e-6 of the state's norm after thousands of tokens); keys,
 // queries and values are bf16 as they come, their norms factors outside. What only an
 // output sees (S0 beside the queries, P) goes in one term, 2^-9, like the output itself.
-// Three terms would cost half as many products again.
+// Three terms would cost half as many products again. So the state is off by 2e-6 to 5e-6 of
+// its norm where fp32 products leave 2e-7 to 4e-7, and outputs by 2.3e-3 where one
+// rounding leaves 1.7e-3; one token at a time (the step) is fp32 throughout.
 //
 // What bounds it. The state passes from chunk to chunk, so a sequence of 2048 tokens is 32
-// steps of 2.4 us however much of the GPU is free (92 us in all, 75 of them the walk);
+// steps of 2.4 us however much of the GPU is free (93 us in all, 75 of them the walk);
 // of a step's 4400 cycles 2500 are tensor (316 products of 8 in the first warp of a pair),
 // the rest the splitting, the short dependent products of the solve, and their operands. 64
-// ragged prompts of 32 heads (17.5k tokens) take 537 us: the walk 413 at 0.60 of the
-// rate of mma.sync and 0.33 of HBM's, the first kernel 124. tcgen05 was not taken: the
-// state would go through tensor memory and registers five times a chunk (state, R, N and
-// their terms), 500 columns of 32 lanes and about 2000 instructions a thread, as long as
-// the walk takes now at a few percent of that unit.
+// ragged prompts of 32 heads (17.5k tokens) take 535 us: the walk 410 at 0.60 of the
+// rate of mma.sync and 0.33 of HBM's, the first kernel 125. tcgen05, with three times that
+// rate, has not been tried: the state would go through tensor memory and registers five
+// times a chunk (state, R, N and their terms), 500 columns of 32 lanes and about 2000
+// instructions a thread, against the 12000 cycles that a chunk and head take of an SM now.
 #include "d3_common.cuh"
 #include "d3_host.h"
 #include "mma_tiles.cuh"
@@ -303,9 +305,10 @@ __device__ __forceinline__ void prep_elements(const float (&acc)[8][4], int head
 }
 
 // One CTA per (record, key head), two of its value heads at a time: bound by latency and
-// instructions, not by its 278 MB (124 us for 305 chunks of 16 key heads, 45% of issue
-// slots busy with four CTAs on an SM). Warps 0-3 make
-// k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads share them.
+// instructions, not by its 278 MB (125 us for 305 chunks of 16 key heads, 45% of issue
+// slots busy with four CTAs on an SM, for which it is held at 64 registers: 8 bytes are
+// spilled). Warps 0-3 make k_i.k_j, warps 4-7 q_i.k_j, each for 16 rows; the two heads
+// share them.
 template <int DK>
 __global__ void __launch_bounds__(kPrepThreads, 4) gated_delta_prep_kernel(const ChunkArgs a) {
   using Sh = PrepShape<DK>;
@@ -618,7 +621,7 @@ __device__ __noinline__ void delta_tokens(float (&s)[DK / 8][4], const DeltaArgs
 // beside it that takes what the next chunk does not wait for, the loads, S0^T q, P N and the
 // output. It gets the state's first terms and N as the A operands they are, through
 // shared memory (two named barriers a chunk). 2048 tokens of one sequence: 125 us without, 118
-// with 64 columns, 92 with 32, where each warp has a scheduler and its tensor unit to itself.
+// with 64 columns, 93 with 32, where each warp has a scheduler and its tensor unit to itself.
 // With many CTAs it would only take the place of a second CTA's warps.
 template <int DK, int DV, bool PAIR, int W>
 __global__ void __launch_bounds__(32 * W * (PAIR ? 2 : 1), PAIR ? 1 : 2) gated_delta_walk_kernel(const ChunkArgs a) {

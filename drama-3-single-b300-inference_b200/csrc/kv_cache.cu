@@ -2,8 +2,8 @@
 // copies of whole pages (forks, compaction). Both move each byte once in and
 // once out, so they are bound by HBM (or, for a decode step, by launch latency):
 // 1500 pages of 16 KB in 20 planes, 983 MB, are copied in 149 us, 6.6 TB/s, the rate of
-// a plain copy; 15670 tokens of 2 x 2 x 256 are appended in 12.9 us, 5.0 TB/s; 64 tokens in
-// 2.4 us, 16 pages in 20 planes in 3.8 us.
+// a plain copy; 15670 tokens of 2 x 2 x 256 are appended in 13.1 us, 4.9 TB/s; 64 tokens in
+// 2.6 us, 16 pages in 20 planes in 2.9 us.
 #include "kv_cache.cuh"
 
 namespace d3 {

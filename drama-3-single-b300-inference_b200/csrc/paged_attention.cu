@@ -19,8 +19,8 @@
 // 131k tokens, 977 MB, in 162 us, 6.04 TB/s or 0.93 of the copy rate (a split of the line
 // into more CTAs than fit at once, deeper rings and prefetches to L2 were all slower; SMs
 // do not get equal shares of the bandwidth, and the slowest ends the kernel); 64 of up to
-// 2048, 136 MB, in 33 us, of which start and joining take about 10; 1 of 301 in 7.1 us. 16
-// of up to 16411 in e4m3 (32 query and 8 key heads of 128), 311 MB: 63 us, 4.9 TB/s, issue
+// 2048, 136 MB, in 33 us, of which start and joining take about 10; 1 of 301 in 7.5 us. 16
+// of up to 16411 in e4m3 (32 query and 8 key heads of 128), 311 MB: 64 us, 4.9 TB/s, issue
 // slots 0.53 busy with widening and twice the products per byte.
 //
 // Inside a CTA 4 warps run on their own: warp w takes keys [w*NK, (w+1)*NK) of a
@@ -77,7 +77,8 @@ struct AttnArgs {
 
 constexpr int attn_ctas(int D, int elem) { return D * elem >= 256 ? 2 : 3; }
 
-// Sizes of one variant. WIDE: 16 query heads per unit, else 8.
+// Sizes of one variant. WIDE: 16 query heads per unit, else 8. (e4m3 with 256 columns and WIDE
+// spills 34 bytes at 255 registers; no other variant of the main kernel does.)
 template <int DT, int D, bool WIDE>
 struct AttnShape {
   static constexpr int kElem = DT == D3_DTYPE_E4M3 ? 1 : 2;
@@ -804,9 +805,15 @@ __global__ void __launch_bounds__(32 * WARPS) paged_attention_join_kernel(const 
 
 // How units of up to `tiles` tiles each are taken: by clusters of the returned number of
 // CTAs (1: whole), or 0: all units' tiles as one line. Measured in us (bf16, 2 key heads of
-// 256, tiles of 64): 1 sequence of 256 tokens by a cluster 7.0, as a line 9.1, of 1024 9.0
-// and 10.8; 64 sequences of up to 256 whole 10.1, as a line 13.4, of up to 1024 as a line
-// 23.4, whole about 30.
+// 256, tiles of 64): 1 sequence of 256 tokens by a cluster 7.0, as a line 8.7, of 1024 9.0
+// and 9.4; 64 sequences of up to 256 whole 10.1, as a line 13.4, of up to 1024 as a line
+// 23.4, whole about 30. The rule counts tiles for all types and dims. Each form beside the
+// others for 1 to 64 sequences of 2 to 32 tiles, all as long as the bound, with heads of 64, 128
+// and 256 in bf16, of 128 and 256 in e4m3 (tiles of 64 and of 128 keys), 246 cells: its choice
+// is the best form or within 5% of it in 204, within 10% in 224. Where it is not: 8 to 16 tiles
+// of many sequences (64 of 512 tokens, heads of 256: line 21.6, whole 17.2; the line is there for
+// ragged lengths, which the host does not know), and 16 to 24 tiles of one sequence with short
+// rows (24 tiles, 2 heads of 64: cluster 8.3, line 6.5).
 int unit_ctas(int tiles, int64_t units, int grid) {
   if (tiles <= 2 || (tiles <= 6 && units * 4 >= grid)) return 1;  // short, or enough of them to fill the GPU
   int n = 8;

@@ -29,7 +29,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     positions[t] (int32) of sequence seq_ids[t] (int32; None: sequence t);
     negative ones are skipped. An e4m3 cache takes bf16 rows and holds
     e4m3(clamp(x / scale[head], -448, 448)). Tokens past the table or on a page
-    outside the cache are not written and set status to D3_STATUS_BAD_ROW."""
+    outside the cache are not written and set status to D3_STATUS_BAD_ROW. No two
+    tokens of a call may name one place."""
     _lib.native().kv_append(k, v, k_cache, v_cache, page_table, positions, seq_ids, k_scale, v_scale, status)
 
 
@@ -48,7 +49,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """softmax(scale * q K^T) V for one new token per sequence: q [B, heads,
     dim], over the first seq_lens[b] (int32) cached tokens, or the last `window`
     of them. scale: dim**-0.5 by default. max_seq_len bounds seq_lens on the host
-    (default: what the page table can hold). Returns out (q's dtype), or (out,
+    (default: what the page table can hold); tokens past it are not read. A page
+    number outside the cache is read as page 0, with status set to
+    D3_STATUS_BAD_ROW. Returns out (q's dtype), or (out,
     lse f32 [B, heads]) with return_lse. An empty sequence gives zeros and
     lse = -inf. Nothing is read on the host, so the call can be captured."""
     return _lib.native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, scale, k_scale, v_scale, window,

@@ -27,7 +27,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     """One token for each of n sequences: q, k bf16 [n, key_heads, key_dim], v
     bf16 [n, value_heads, value_dim], g (log decay) and beta f32 [n,
     value_heads]. Sequence i's state is state[slots[i]] (int32; None: state[i]),
-    updated in place; a negative slot leaves the sequence out (zero row). q and
+    updated in place; a negative slot leaves the sequence out (zero row), and no
+    two sequences of a call may share one. q and
     k are divided by sqrt(|x|^2 + eps) when l2norm; scale: key_dim**-0.5 by
     default. Returns out bf16 [n, value_heads, value_dim]."""
     return _lib.native().gated_delta_step(q, k, v, g, beta, state, slots, scale, l2norm, eps, out, status)
@@ -52,7 +53,12 @@ def gated_delta_chunk(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     sequence i's tokens. Each sequence starts from state[slots[i]] (None:
     state[i]), or from zero where fresh[i] (bool [n]), and leaves its state
     there. Other arguments and the result are those of gated_delta_step; out must
-    not overlap q, k or v. The lengths are read on the device, so the call can be
-    captured."""
+    not overlap q, k or v, and its rows of no sequence are not written. The lengths
+    are read on the device, so the call can be captured.
+
+    Chunks of 64 tokens are multiplied with two bf16 terms per factor: the fp32
+    state is within 2**-16 of its norm of the rule (2e-6 to 5e-6 measured), where
+    gated_delta_step, all in fp32, keeps 2**-20, and out is rounded once more than
+    there (2.3e-3 of its norm against 1.7e-3)."""
     return _lib.native().gated_delta_chunk(q, k, v, g, beta, state, cu_seqlens, slots, fresh, scale, l2norm, eps, out,
                                            workspace, status)
